@@ -154,7 +154,8 @@ B2_API int b2_dequantize_matmul_noalloc(const b2_tensor *a, const b2_tensor *w,
  * when none, else the first code found (1: data never arrived, 2: a ring slot
  * never freed, 3: an MMA never completed), with the kernel named in
  * b2_last_error(); 4 when b2_rotary_embedding met a position_ids value
- * outside its cos/sin cache (the reference throws there; those outputs are 0).
+ * outside its cos/sin cache (the reference throws there; those outputs are 0),
+ * or an operator on the 8-bit cache a length or page number out of range.
  * A call whose kernel gave up leaves its output unwritten (or partly written)
  * and is reported only here.  The codes live in device
  * words of the library, never in a caller's workspace.  Synchronizes the
@@ -308,6 +309,104 @@ B2_API int b2_rotary_embedding(const b2_tensor *x, const b2_tensor *cos_cache,
  */
 B2_API int b2_swiglu(const b2_tensor *a, const b2_tensor *b, float alpha, b2_tensor *y,
                      void *stream);
+
+/*
+ * A decoder step with 8-bit activations and an 8-bit KV cache.  Codes are INT8
+ * (|code| <= 127) or FLOAT8E4M3FN (|code| <= 448) and stand for code * scale;
+ * the scale of a group of values is its largest magnitude / 127 or / 448, the
+ * code round(value / scale), nearest even.  A group of zeros has scale 0; a
+ * NaN or an infinity in a group makes its scale NaN or infinite and leaves no
+ * NaN code.  No counterpart in onnx-light.
+ */
+
+/*
+ * RMS normalization with the residual's addition and an 8-bit output:
+ *   h = x + residual;  n = h / sqrt(mean(h^2 over the last axis) + epsilon) * scale
+ *   y_scale = max |n| / 127 or 448 per group;  y = round(n / y_scale)
+ *  x: FLOAT, FLOAT16 or BFLOAT16 [..., C]; residual: NULL or x's dtype and shape;
+ *  scale: x's dtype, [C]; group_size: 0 (one group per row) or a divisor of C;
+ *  y: INT8 or FLOAT8E4M3FN, x's shape; y_scale: FLOAT [..., groups];
+ *  sum: NULL, or h rounded to x's dtype (may be x's or residual's own buffer).
+ * All arithmetic is fp32 and the norm is taken of the unrounded h.
+ */
+B2_API int b2_rms_normalization_quantize(const b2_tensor *x, const b2_tensor *residual,
+                                         const b2_tensor *scale, float epsilon,
+                                         int64_t group_size, b2_tensor *y, b2_tensor *y_scale,
+                                         b2_tensor *sum, void *stream);
+
+/*
+ * Product of two 8-bit operands with scales:
+ *   y[m, n] = a_scale[m] * w_scale[n] * sum_k a[m, k] * w[n, k]
+ *  a: INT8 or FLOAT8E4M3FN [..., K]; w: the same dtype, [N, K] (K innermost);
+ *  a_scale: FLOAT, one value or one per row of a; w_scale: FLOAT, one value or
+ *  one per row of w; y: FLOAT, FLOAT16 or BFLOAT16 [..., N].
+ * INT8 sums are exact (K up to 131071), FLOAT8E4M3FN sums fp32; the scales
+ * multiply the sum in fp32 and the result is rounded once.
+ */
+B2_API int b2_scaled_matmul(const b2_tensor *a, const b2_tensor *a_scale, const b2_tensor *w,
+                            const b2_tensor *w_scale, b2_tensor *y, void *workspace,
+                            size_t *workspace_bytes, void *stream);
+
+/*
+ * A paged KV cache held in 8 bits.  Position p of sequence b lies in row
+ * p % page_size of page block_table[b][p / page_size]; every page and KV head
+ * has one scale for its keys and one for its values.
+ *  k, v: INT8 or FLOAT8E4M3FN [pages, kv_heads, page_size, head_size];
+ *  k_scale, v_scale: FLOAT [pages, kv_heads];
+ *  block_table: INT32 [batch, max_pages]; lengths: INT32 [batch], the tokens
+ *  each sequence holds before the call (the calls do not change it).
+ * Pages past a sequence's tokens are never read, whatever the table holds
+ * there.  A page that gets new tokens belongs to one sequence.
+ */
+typedef struct b2_quantized_cache {
+  const b2_tensor *k, *v, *k_scale, *v_scale, *block_table, *lengths;
+} b2_quantized_cache;
+
+/*
+ * Appends new keys and values at positions lengths[b] .. lengths[b] +
+ * new_lengths[b] - 1 of each sequence.
+ *  k, v: FLOAT, FLOAT16 or BFLOAT16, [batch, kv_heads, new, head_size] or
+ *    [batch, new, kv_heads * head_size];
+ *  new_lengths: NULL (all `new`) or INT32 [batch], the rows of k and v that count.
+ * A page's scale covers all its tokens: s' = max(s, max |new| / 127 or 448),
+ * with s the scale of the tokens the page already holds of this sequence (0
+ * when it holds none); where s' > s, their codes become round(code * (s / s')).
+ * Tokens past the table, and pages numbered outside the pool, are not written;
+ * b2_kernel_status reports either.
+ */
+B2_API int b2_kv_cache_append(const b2_tensor *k, const b2_tensor *v,
+                              const b2_quantized_cache *cache, const b2_tensor *new_lengths,
+                              void *stream);
+
+typedef struct b2_cache_attention_attrs {
+  int32_t has_scale; /* 0: scale = 1/sqrt(head_size) */
+  float scale;
+  int32_t is_causal; /* 0: every key of the sequence is seen */
+  float softcap;     /* > 0: softcap * tanh(s / softcap) before the mask */
+  int64_t left_window_size; /* -1: unbounded; else keys up to this far before the query (causal only) */
+  int64_t sink_tokens;      /* first tokens that stay visible outside the window */
+} b2_cache_attention_attrs;
+
+/*
+ * Attention of new queries over the cache, after b2_kv_cache_append of the
+ * same tokens: query i of sequence b stands at position p = lengths[b] + i and
+ * sees the keys j < lengths[b] + new_lengths[b] with j <= p (causal) and, with
+ * a window, p - j <= left_window_size or j < sink_tokens.
+ *  q: FLOAT16 or BFLOAT16, [batch, heads, new, head_size] or [batch, new,
+ *    heads * head_size], heads a multiple of the cache's kv_heads;
+ *  new_lengths: as in b2_kv_cache_append; y: q's dtype and shape.
+ * A query that sees no key, and every row past new_lengths[b], gives 0.
+ * Scores, softmax and sums are fp32.  Codes in rows that hold no token of the
+ * sequence are never used, whatever they are; within its tokens a
+ * FLOAT8E4M3FN code must be a number (b2_kv_cache_append writes no other; a
+ * NaN among the values is carried by the page's scale).  Lengths past the table
+ * are cut to it and pages numbered outside the pool are skipped;
+ * b2_kernel_status reports either.
+ */
+B2_API int b2_cache_attention(const b2_tensor *q, const b2_quantized_cache *cache,
+                              const b2_tensor *new_lengths,
+                              const b2_cache_attention_attrs *attrs, b2_tensor *y,
+                              void *workspace, size_t *workspace_bytes, void *stream);
 
 /*
  * Multi-GPU support: device buffers shared between the processes of a group

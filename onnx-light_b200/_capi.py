@@ -47,7 +47,8 @@ EXPORTS = ("b2_version", "b2_last_error", "b2_dequantize_linear", "b2_dequantize
            "b2_rms_normalization", "b2_rotary_embedding", "b2_swiglu", "b2_ipc_alloc",
            "b2_ipc_free", "b2_ipc_open", "b2_ipc_close", "b2_allgather_cols",
            "b2_dequantize_matmul_peer", "b2_peer_wait", "b2_dequantize_matmul_group",
-           "b2_dequantize_matmul_group_peer")
+           "b2_dequantize_matmul_group_peer", "b2_rms_normalization_quantize", "b2_scaled_matmul",
+           "b2_kv_cache_append", "b2_cache_attention")
 
 
 class B2Tensor(C.Structure):
@@ -68,6 +69,18 @@ class B2AttentionAttrs(C.Structure):
                 ("q_num_heads", C.c_int64), ("kv_num_heads", C.c_int64),
                 ("left_window_size", C.c_int64), ("right_window_size", C.c_int64),
                 ("kv_capacity", C.c_int64)]
+
+
+class B2QuantizedCache(C.Structure):
+    """b2_quantized_cache: the tensors of a paged 8-bit KV cache."""
+    _fields_ = [(n, C.POINTER(B2Tensor)) for n in ("k", "v", "k_scale", "v_scale", "block_table",
+                                                   "lengths")]
+
+
+class B2CacheAttentionAttrs(C.Structure):
+    _fields_ = [("has_scale", C.c_int32), ("scale", C.c_float), ("is_causal", C.c_int32),
+                ("softcap", C.c_float), ("left_window_size", C.c_int64),
+                ("sink_tokens", C.c_int64)]
 
 
 class B2Error(RuntimeError):
@@ -125,6 +138,12 @@ def lib() -> C.CDLL:
                 L.b2_dequantize_matmul_group.argtypes = [C.c_int32, T, T, T, C.c_int64, T, P, SZ, P]
                 L.b2_dequantize_matmul_group_peer.argtypes = [C.c_int32, T, T, T, C.c_int64, T,
                                                               C.POINTER(B2PeerOut), P, SZ, P]
+                QC = C.POINTER(B2QuantizedCache)
+                L.b2_rms_normalization_quantize.argtypes = [T, T, T, C.c_float, C.c_int64, T, T, T, P]
+                L.b2_scaled_matmul.argtypes = [T, T, T, T, T, P, SZ, P]
+                L.b2_kv_cache_append.argtypes = [T, T, QC, T, P]
+                L.b2_cache_attention.argtypes = [T, QC, T, C.POINTER(B2CacheAttentionAttrs), T, P,
+                                                 SZ, P]
                 L.b2_synth_fill.argtypes = [C.c_int32, C.c_uint64, C.c_int64, C.c_double,
                                             C.c_double, P, P]
                 L.b2_convert.argtypes = [P, C.c_int32, P, C.c_int32, C.c_int64, P]

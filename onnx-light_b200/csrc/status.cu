@@ -29,6 +29,8 @@ int status_read_dq_gemm_f32(int reset);
 int status_read_gemv_x(int reset);
 int status_read_gemv_n(int reset);
 int status_read_gemv_c(int reset);
+int status_read_cache_append(int reset);
+int status_read_cache_attention(int reset);
 
 __device__ int g_selftest_status;
 
@@ -55,6 +57,7 @@ extern "C" B2_API int b2_kernel_status(int reset) {
   // code: the kernels' time-out codes (1..3), or kOutOfRange for an input
   // value a device kernel could not reject on the host
   constexpr int kOutOfRange = 4;
+  constexpr int kCacheRange = 5; // reported as kOutOfRange, with its own message
   struct Src { const char *name; int (*read)(int); int code; };
   const Src srcs[] = {{"dq_gemv_mma", status_read_gemv_mma, 0},
                       {"dq_gemv_x", status_read_gemv_x, 0},
@@ -68,15 +71,20 @@ extern "C" B2_API int b2_kernel_status(int reset) {
                       {"dq_gemv_i4h", status_read_dq_gemv, 0},
                       {"dq_gemm_f32", status_read_dq_gemm_f32, 0},
                       {"allgather_cols", status_read_allgather, 0},
-                      {"kernel::RotaryEmbedding", status_read_rotary, kOutOfRange}};
+                      {"kernel::RotaryEmbedding", status_read_rotary, kOutOfRange},
+                      {"b200::KVCacheAppend", status_read_cache_append, kCacheRange},
+                      {"b200::QuantizedCacheAttention", status_read_cache_attention, kCacheRange}};
   int first = 0;
   for (const Src &s : srcs) {
     const int v = s.read(reset);
     if (v < 0) B2_FAIL(B2_ERR_CUDA, "b2_kernel_status: reading the status of %s failed", s.name);
     if (v && !first) {
-      first = s.code ? s.code : v;
+      first = s.code ? kOutOfRange : v;
       if (s.code == kOutOfRange)
         set_error(B2_OK, "%s: position_ids value out of range (those outputs were written as 0)",
+                  s.name);
+      else if (s.code == kCacheRange)
+        set_error(B2_OK, "%s: a length or page number of the cache was out of range (those tokens were skipped)",
                   s.name);
       else
         set_error(B2_OK, "%s: a bounded wait timed out (code %d: %s)", s.name, v,

@@ -24,15 +24,16 @@ from __future__ import annotations
 
 from typing import Callable, Dict, Optional
 
-from .kernels import (Attention, DequantizeLinear, DequantizeMatMul, MatMulInteger,
-                      QLinearMatMul, RMSNormalization, RotaryEmbedding, SwiGLU)
+from .kernels import (Attention, DequantizeLinear, DequantizeMatMul, KVCacheAppend, MatMulInteger,
+                      QLinearMatMul, QuantizedCacheAttention, RMSNormalization,
+                      RMSNormalizationQuantize, RotaryEmbedding, ScaledMatMul, SwiGLU)
 
 K_DEFAULT_ONNX_DOMAIN = "ai.onnx"
 DEVICE_CPU = -1
 DEVICE_UNDEFINED = -2
 DEVICE_GPU0 = 0
 MAX_GPU_INDEX = 8191
-FUSED_DOMAIN = "b200"  # custom domain of the fused DequantizeLinear -> MatMul node
+FUSED_DOMAIN = "b200"  # custom domain of the operators onnx-light has no node for
 
 
 def normalise_domain(domain: str) -> str:
@@ -103,6 +104,10 @@ def RegisterB200KernelFunctions(table: Optional[KernelDispatchTable] = None,
         ("", "RotaryEmbedding"): RotaryEmbedding,
         ("", "SwiGLU"): SwiGLU,
         (FUSED_DOMAIN, "DequantizeMatMul"): DequantizeMatMul,
+        (FUSED_DOMAIN, "RMSNormalizationQuantize"): RMSNormalizationQuantize,
+        (FUSED_DOMAIN, "ScaledMatMul"): ScaledMatMul,
+        (FUSED_DOMAIN, "KVCacheAppend"): KVCacheAppend,
+        (FUSED_DOMAIN, "QuantizedCacheAttention"): QuantizedCacheAttention,
     }
     for i in range(num_gpus):
         for (domain, op), cls in entries.items():

@@ -390,3 +390,196 @@ class SwiGLU:
         ad, bd, yd = _desc(a), _desc(b), _desc(out)
         check(lib().b2_swiglu(ad.ref, bd.ref, float(alpha), yd.ref, stream_ptr(a.device)))
         return out
+
+
+# ---------------------------------------------------------------------------
+# A decoder step with 8-bit activations and an 8-bit KV cache.  Codes are INT8
+# (torch.int8 tensors) or FLOAT8E4M3FN (QTensor over uint8 storage) and stand
+# for code * scale.  No counterpart in onnx-light.
+# ---------------------------------------------------------------------------
+
+
+def _new_codes(shape, dtype: int, device):
+    """An uninitialised tensor of 8-bit codes: torch.int8, or a QTensor of FLOAT8E4M3FN."""
+    if dtype == capi.INT8:
+        return torch.empty(shape, dtype=torch.int8, device=device)
+    if dtype == capi.FLOAT8E4M3FN:
+        return QTensor(torch.empty(shape, dtype=torch.uint8, device=device), dtype, tuple(shape))
+    raise ValueError("8-bit codes are INT8 or FLOAT8E4M3FN")
+
+
+@dataclass
+class QuantizedNorm:
+    Y: object  # codes: torch.int8, or a QTensor of FLOAT8E4M3FN
+    Y_scale: torch.Tensor
+    sum: Optional[torch.Tensor] = None
+
+
+class RMSNormalizationQuantize:
+    """RMS normalization of ``x + residual`` with an 8-bit output and scales.
+
+    ``h = x + residual``, ``n = h / sqrt(mean(h^2) + epsilon) * scale`` over the last axis,
+    ``Y_scale = max |n| / 127`` (INT8) or ``/ 448`` (FLOAT8E4M3FN) per row or per ``group_size``
+    columns, ``Y = round(n / Y_scale)``.  With a residual the result also carries ``sum``: h in x's
+    dtype, the next layer's residual.  Y * Y_scale is what DequantizeLinear (blocked along the last
+    axis) or ScaledMatMul (one group per row) make of it.
+    """
+
+    name = "onnx_kernels:GPU:b200:RMSNormalizationQuantize"
+
+    def __call__(self, x: torch.Tensor, scale: torch.Tensor,
+                 residual: Optional[torch.Tensor] = None, epsilon: float = 1e-5,
+                 dtype: int = capi.FLOAT8E4M3FN, group_size: int = 0, out=None,
+                 out_scale: Optional[torch.Tensor] = None,
+                 out_sum: Optional[torch.Tensor] = None) -> QuantizedNorm:
+        shape = tuple(x.shape)
+        if out is None:
+            out = _new_codes(shape, dtype, x.device)
+        if out_scale is None:
+            if group_size < 0 or (group_size and shape[-1] % group_size):
+                raise ValueError("b200::RMSNormalizationQuantize: group_size must divide the number "
+                                 "of columns (0: one group per row).")
+            out_scale = torch.empty(shape[:-1] + (shape[-1] // group_size if group_size else 1,),
+                                    dtype=torch.float32, device=x.device)
+        if out_sum is None and residual is not None:
+            out_sum = torch.empty_like(x)
+        xd, sd, yd, ysd = _desc(x), _desc(scale), _desc(out), _desc(out_scale)
+        rd = _desc(residual) if residual is not None else None
+        hd = _desc(out_sum) if out_sum is not None else None
+        check(lib().b2_rms_normalization_quantize(xd.ref, _ref(rd), sd.ref, float(epsilon),
+                                                  int(group_size), yd.ref, ysd.ref, _ref(hd),
+                                                  stream_ptr(x.device)))
+        return QuantizedNorm(out, out_scale, out_sum)
+
+
+class ScaledMatMul:
+    """``y[m, n] = a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k]`` of two 8-bit operands.
+
+    ``a`` [..., K] and ``w`` [N, K] are both INT8 or both FLOAT8E4M3FN; the scales hold one value or
+    one per row.  INT8 sums are exact; the result is rounded once, to ``dtype``.
+    """
+
+    name = "onnx_kernels:GPU:b200:ScaledMatMul"
+
+    def __call__(self, a, a_scale: torch.Tensor, w, w_scale: torch.Tensor,
+                 dtype: torch.dtype = torch.float16,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if out is None:
+            out = torch.empty(tuple(a.shape[:-1]) + (int(w.shape[0]),), dtype=dtype,
+                              device=a.device)
+        ad, asd, wd, wsd, yd = _desc(a), _desc(a_scale), _desc(w), _desc(w_scale), _desc(out)
+        _call_with_workspace(lib().b2_scaled_matmul,
+                             (ad.ref, asd.ref, wd.ref, wsd.ref, yd.ref),
+                             (stream_ptr(out.device),), out.device)
+        return out
+
+
+class QuantizedKVCache:
+    """Paged KV cache in 8 bits: pages of ``page_size`` tokens with one scale per page and KV head.
+
+    ``k`` / ``v``: [pages, kv_heads, page_size, head_size] codes (torch.int8, or uint8 storage of
+    FLOAT8E4M3FN); ``k_scale`` / ``v_scale``: FLOAT [pages, kv_heads]; ``block_table``: INT32
+    [batch, max_pages], the page of each sequence's positions; ``lengths``: INT32 [batch], the
+    tokens held.  The operators read ``lengths`` and do not change it: a step appends and attends in
+    every layer with the same lengths, then calls :meth:`advance` once.
+    """
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor,
+                 v_scale: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+                 dtype: int):
+        if dtype not in (capi.INT8, capi.FLOAT8E4M3FN):
+            raise ValueError("QuantizedKVCache: dtype must be INT8 or FLOAT8E4M3FN")
+        if k.element_size() != 1 or v.element_size() != 1:
+            raise ValueError("QuantizedKVCache: k and v must hold 8-bit codes")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.block_table, self.lengths, self.dtype = block_table, lengths, dtype
+
+    @classmethod
+    def allocate(cls, batch: int, kv_heads: int, capacity: int, head_size: int,
+                 page_size: int = 64, dtype: int = capi.FLOAT8E4M3FN, device="cuda", pages=None,
+                 block_table: Optional[torch.Tensor] = None) -> "QuantizedKVCache":
+        """An empty cache of ``capacity`` tokens per sequence.  Without a ``block_table`` sequence b
+        owns the pages from b * max_pages on."""
+        per = -(-capacity // page_size)
+        if block_table is None:
+            block_table = torch.arange(batch * per, dtype=torch.int32, device=device).view(batch, per)
+        pages = batch * per if pages is None else pages
+        kind = torch.int8 if dtype == capi.INT8 else torch.uint8
+        k, v = (torch.zeros((pages, kv_heads, page_size, head_size), dtype=kind, device=device)
+                for _ in range(2))
+        ks, vs = (torch.zeros((pages, kv_heads), dtype=torch.float32, device=device)
+                  for _ in range(2))
+        return cls(k, v, ks, vs, block_table,
+                   torch.zeros(batch, dtype=torch.int32, device=device), dtype)
+
+    def advance(self, new_lengths) -> None:
+        """Counts the tokens of a finished step (an int, or INT32 [batch])."""
+        self.lengths += new_lengths
+
+    def _descs(self):
+        """The struct of the C call and what keeps it alive."""
+        ds = [_desc(self.k, self.dtype), _desc(self.v, self.dtype), _desc(self.k_scale),
+              _desc(self.v_scale), _desc(self.block_table), _desc(self.lengths)]
+        return capi.B2QuantizedCache(*[C.pointer(d.t) for d in ds]), ds
+
+
+class KVCacheAppend:
+    """Writes new keys and values behind the tokens a :class:`QuantizedKVCache` holds.
+
+    ``K`` / ``V``: [batch, kv_heads, new, head_size] or [batch, new, kv_heads * head_size];
+    ``new_lengths``: INT32 [batch], how many rows of each sequence count (all without it).  A page's
+    scale covers all its tokens and grows when a new one needs it; the older codes of that page are
+    then rounded once more.
+    """
+
+    name = "onnx_kernels:GPU:b200:KVCacheAppend"
+
+    def __call__(self, K: torch.Tensor, V: torch.Tensor, cache: QuantizedKVCache,
+                 new_lengths: Optional[torch.Tensor] = None) -> None:
+        kd, vd = _desc(K), _desc(V)
+        nd = _desc(new_lengths) if new_lengths is not None else None
+        cd, keep = cache._descs()
+        check(lib().b2_kv_cache_append(kd.ref, vd.ref, C.byref(cd), _ref(nd),
+                                       stream_ptr(K.device)))
+
+
+@dataclass
+class CacheAttributes:
+    """Attributes of QuantizedCacheAttention; with a window, ``sink_tokens`` first tokens stay
+    visible to every query."""
+
+    has_scale: bool = False
+    scale: float = 0.0
+    is_causal: bool = True
+    softcap: float = 0.0
+    left_window_size: int = -1
+    sink_tokens: int = 0
+
+
+class QuantizedCacheAttention:
+    """Attention of new queries over a :class:`QuantizedKVCache` that already holds their keys.
+
+    ``Q``: FLOAT16 / BFLOAT16 [batch, heads, new, head_size] or [batch, new, heads * head_size];
+    query i of sequence b stands at position lengths[b] + i.  Call after KVCacheAppend of the same
+    tokens and before ``cache.advance``.  Rows past ``new_lengths`` give 0.
+    """
+
+    name = "onnx_kernels:GPU:b200:QuantizedCacheAttention"
+
+    def __call__(self, Q: torch.Tensor, cache: QuantizedKVCache,
+                 attrs: Optional[CacheAttributes] = None,
+                 new_lengths: Optional[torch.Tensor] = None,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        attrs = attrs or CacheAttributes()
+        a = capi.B2CacheAttentionAttrs(int(attrs.has_scale), float(attrs.scale),
+                                       int(attrs.is_causal), float(attrs.softcap),
+                                       int(attrs.left_window_size), int(attrs.sink_tokens))
+        if out is None:
+            out = torch.empty_like(Q)
+        qd, yd = _desc(Q), _desc(out)
+        nd = _desc(new_lengths) if new_lengths is not None else None
+        cd, keep = cache._descs()
+        _call_with_workspace(lib().b2_cache_attention,
+                             (qd.ref, C.byref(cd), _ref(nd), C.byref(a), yd.ref),
+                             (stream_ptr(Q.device),), Q.device)
+        return out
