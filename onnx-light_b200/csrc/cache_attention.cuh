@@ -41,4 +41,9 @@ __device__ __forceinline__ bool ca_sees(const CaArgs &a, int p, int j) {
   return j <= p && (a.window < 0 || p - j <= a.window || j < a.sinks);
 }
 
+// Few query rows, keys split over the GPU (cache_attention_split.cu).
+bool cache_attn_split_eligible(const CaArgs &a);
+size_t cache_attn_split_workspace(const CaArgs &a);
+int cache_attn_split_launch(const CaArgs &a, bool f16, bool f8, void *ws, cudaStream_t st);
+
 } // namespace b2

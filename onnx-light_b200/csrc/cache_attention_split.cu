@@ -1,0 +1,828 @@
+// Attention over a paged 8-bit KV cache for few query rows: single tokens and short runs of them
+// (b2_cache_attention), with the keys split over the whole GPU.
+//
+// Bound: HBM, the visible codes of K and V once; for one short sequence, latency.
+//
+// A KV head's queries -- the heads of its group times the new positions, a pack of 8 NT rows -- are
+// the 8-wide N side of mma.sync m16n8k16 and the tokens (Q.K) or head columns (P.V) its 16-row M side,
+// so a code read from HBM serves all of them and no MMA row is padding:
+//   S^T[16 tokens x 8 rows] += K[16 x 16 columns] Q^T     O^T[16 columns x 8 rows] += V^T[16 x 16 tokens] P^T
+// Codes become FLOAT16 in registers, exactly (INT8 and FLOAT8E4M3FN values both fit), and the page
+// scales multiply in fp32: the key scale the score, the value scale the probability.  Sums and the
+// softmax state are fp32.  Three roundings to FLOAT16 remain: BFLOAT16 queries, after a power of two
+// per row brings them to [-2, 2) (8 significant bits fit in 11; columns 2^-14 below the row's largest
+// lose low bits); and p * v_scale, relative to the largest such product of the row, so 2^-11 of
+// what it contributes.  The denominator sums the unrounded p.
+//
+// The running reference of a row is m = max_j (s_j + log2 v_scale_j): with p_j = 2^(s_j - m + 15) in
+// fp32, p_j v_scale_j is at most 2^15 for every token, however far the pages' scales lie apart, and
+// keeps its 11 bits down to 2^-29 of the largest (FLOAT16's normal range ends at 2^-14).  log2
+// v_scale is held to [-60, 110] so that p cannot overflow; a scale below only makes its products
+// smaller.
+//
+// Data path: tiles of 32 tokens (K and V, [32][128 B] with the 128-byte swizzle) through a TMA ring
+// filled by one producer warp.  Page numbers and scales are fetched for the next 8 to 32 tiles at
+// once, one page chunk a lane; the first tiles' copies start before their scales arrive.  Each
+// tile is one consumer warp's: the swizzle makes the fragment reads (16 bytes a lane) free of
+// bank conflicts, for K along a token's columns and for V across four tokens.
+//
+// Split: (sequence, KV head, pack, tile) units are numbered in order and the CTAs (one per SM) take
+// equal ranges, worked out on the device from the lengths, so ragged batches balance and the host
+// never waits.  A CTA merges its warps' (m, l, O) per pair; a pair that spans CTAs is merged
+// by its last arriver in CTA order, so results do not depend on timing.
+#include <algorithm>
+
+#include "cache_attention.cuh"
+#include "tc_common.cuh"
+
+namespace b2 {
+
+__device__ int g_cache_attn_split_status; // time-out code of a bounded wait
+__device__ int g_cache_attn_split_range;  // 1: a length, count or page number was out of range
+
+namespace {
+
+using namespace q8;
+
+constexpr int CS_KEYS = 32; // tokens per tile
+constexpr float CS_LIFT = 15.0f; // log2 of the largest p * v_scale
+constexpr uint32_t CS_BOX = CS_KEYS * 128; // one 128-byte-wide tile of codes
+constexpr size_t CS_SMEM_MAX = 232448;
+
+template <int DP, int NT> struct CsLayout {
+  static constexpr int NB = DP == 256 ? 2 : 1;            // 128-byte boxes per row
+  static constexpr int WARPS = NT == 1 ? 8 : 4;           // consumers
+  static constexpr int THREADS = (WARPS + 1) * 32;
+  static constexpr uint32_t STAGE = 2 * NB * CS_BOX;      // K boxes, V boxes
+  static constexpr uint32_t MERGE = WARPS * 8 * NT * (DP + 2) * 4;
+  static constexpr uint32_t FIXED = 1024 + MERGE + 4096;  // alignment, merge, barriers, scales
+  // Each stage belongs to one consumer warp (see the parity note in the kernel).
+  static constexpr int STAGES = (int)((CS_SMEM_MAX - FIXED) / STAGE) / WARPS * WARPS < 24
+                                    ? (int)((CS_SMEM_MAX - FIXED) / STAGE) / WARPS * WARPS
+                                    : 24;
+  static constexpr uint32_t OFF_MERGE = STAGES * STAGE;
+  static constexpr uint32_t OFF_BAR = OFF_MERGE + MERGE;  // full, empty
+  static constexpr uint32_t OFF_SC = OFF_BAR + 24 * 16;   // float4 [STAGES][4]
+  static constexpr uint32_t OFF_MISC = OFF_SC + 24 * 64;
+  static constexpr size_t SMEM = OFF_MISC + 256 + 1024;
+  static_assert(STAGES >= WARPS && SMEM <= CS_SMEM_MAX, "shared memory");
+};
+
+struct CsArgs {
+  CaArgs c;
+  int packs, rows;  // packs of 8 NT rows of a KV head's `rows` = S * group
+  int chunk;        // tokens per TMA box: a power of two, 8 to 32, that divides the page
+  int align_pairs;  // CTA ranges start at pair boundaries (more pairs than counters)
+  float *partials;  // [grid][2][8 NT][DP + 2]: O, m, l
+  uint32_t *counters;
+};
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, "
+               "{%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transposes an 8 x 8 matrix of 16-bit elements held one row of pairs a lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Codes in a word -> exact FLOAT16 pairs: bytes 0 and 1 to lo, 2 and 3 to hi.
+template <typename Q> __device__ __forceinline__ void to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  if constexpr (std::is_same<Q, Fp8>::value) {
+    asm("{\n\t.reg .b16 a, b;\n\t"
+        "mov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  } else {
+    // code + 128 as the low byte of 1024 + (code + 128), an exact FLOAT16, minus 1152
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 k = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), k);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2 *>(&b), k);
+    lo = *reinterpret_cast<const uint32_t *>(&x);
+    hi = *reinterpret_cast<const uint32_t *>(&y);
+  }
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+// 16-byte unit u (0..7) of row r in a [rows][128 B] box written with the 128-byte swizzle.
+__device__ __forceinline__ uint32_t unit_at(uint32_t base, int r, int u) {
+  return base + (uint32_t)(r * 128 + ((u ^ (r & 7)) << 4));
+}
+
+// The tiles of sequence b: the window's (from the first query's) and the sinks' before it.
+struct CsSeq {
+  CaSpan sp;
+  int first, sink_tiles, tiles; // first window tile; tiles before it; all tiles (at least 1)
+};
+__device__ __forceinline__ CsSeq cs_seq(const CaArgs &a, int b, bool *bad) {
+  CsSeq s;
+  s.sp = ca_span(a, b, bad);
+  const bool win = a.causal && a.window >= 0;
+  s.first = win ? max(0, s.sp.past - a.window) / CS_KEYS : 0;
+  s.sink_tiles = win ? min((min(a.sinks, s.sp.total) + CS_KEYS - 1) / CS_KEYS, s.first) : 0;
+  s.tiles = s.sp.count > 0 ? s.sink_tiles + (s.sp.total + CS_KEYS - 1) / CS_KEYS - s.first : 0;
+  s.tiles = max(s.tiles, 1); // a sequence without new tokens still gets its zeros written
+  return s;
+}
+__device__ __forceinline__ int cs_key0(const CsSeq &s, int tile) {
+  return (tile < s.sink_tiles ? tile : s.first + tile - s.sink_tiles) * CS_KEYS;
+}
+
+// A walk over the units in order.
+struct CsWalk {
+  int b, before; // sequence, tiles (per pair) of the sequences before it
+  CsSeq s;
+  int pair, tile; // of the unit: KV head * packs + pack, tile
+};
+__device__ __forceinline__ void cs_seek(const CsArgs &g, CsWalk &w, int64_t u) {
+  const int64_t hp = (int64_t)g.c.Hkv * g.packs;
+  bool bad;
+  while (u >= (w.before + (int64_t)w.s.tiles) * hp) {
+    w.before += w.s.tiles;
+    w.s = cs_seq(g.c, ++w.b, &bad);
+  }
+  const int64_t r = u - w.before * hp;
+  w.pair = (int)(r / w.s.tiles);
+  w.tile = (int)(r - (int64_t)w.pair * w.s.tiles);
+}
+// Positions of the pack's first and last query (last < first: none counts).
+__device__ __forceinline__ void cs_pack(const CsArgs &g, const CsSeq &s, int pack, int rows_per_pack,
+                                        int *first, int *last) {
+  const int r0 = pack * rows_per_pack, r1 = min(g.rows, r0 + rows_per_pack) - 1;
+  *first = s.sp.past + r0 / g.c.group;
+  *last = s.sp.past + min(r1 / g.c.group, s.sp.count - 1);
+}
+// Whether any query of the pack may see a key of the tile.
+__device__ __forceinline__ bool cs_live(const CsArgs &g, const CsSeq &s, int first, int last, int key0) {
+  if (last < first || key0 >= s.sp.total) return false;
+  if (!g.c.causal) return true;
+  if (key0 > last) return false;
+  return g.c.window < 0 || key0 + CS_KEYS > first - g.c.window || key0 < g.c.sinks;
+}
+
+// Sum of v over the block and the sum over the threads before this one; every thread calls it.
+template <int THREADS> __device__ __forceinline__ int block_scan(int v, int *total, int *red) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += t;
+  }
+  __syncthreads(); // red is free
+  if (lane == 31) red[warp] = inc;
+  __syncthreads();
+  int base = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    const int t = red[w];
+    if (w < warp) base += t;
+    all += t;
+  }
+  *total = all;
+  return base + inc - v;
+}
+
+__device__ __forceinline__ uint32_t arrive_acq_rel(uint32_t *p, uint32_t v) {
+  uint32_t old;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+  return old;
+}
+
+template <typename T, typename Q, int DP, int NT>
+__global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
+    cache_attn_split(const __grid_constant__ CUtensorMap map_k,
+                     const __grid_constant__ CUtensorMap map_v, const CsArgs g) {
+  using L = CsLayout<DP, NT>;
+  constexpr int STAGES = L::STAGES, WARPS = L::WARPS, NB = L::NB, RP = 8 * NT;
+  constexpr int KS = DP / 16;                 // k16 steps of Q.K; M tiles of P.V
+  extern __shared__ uint8_t dsm[];
+  uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(dsm) + 1023) & ~uintptr_t(1023));
+  uint64_t *full = reinterpret_cast<uint64_t *>(sm + L::OFF_BAR);
+  uint64_t *empty = full + STAGES;
+  float4 *sc = reinterpret_cast<float4 *>(sm + L::OFF_SC);
+  float *mrg = reinterpret_cast<float *>(sm + L::OFF_MERGE);
+  int *misc = reinterpret_cast<int *>(sm + L::OFF_MISC); // [0..15] scan, [16] b, [17] before
+  volatile int *flags = misc + 24;                       // [0] abort [1] last
+  const CaArgs &a = g.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t hp = (int64_t)a.Hkv * g.packs;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1); // one consumer warp per stage
+    }
+    flags[0] = 0;
+    flags[1] = 0;
+    tc::fence_barrier_init();
+  }
+  // ---- this CTA's range of units ----
+  bool bad = false;
+  int64_t tiles_all = 0;
+  int mine = 0, before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += L::THREADS) {
+    const int b = b0 + threadIdx.x;
+    bool bb = false;
+    mine = b < a.B ? cs_seq(a, b, &bb).tiles : 0;
+    bad |= bb;
+    int t;
+    before = block_scan<L::THREADS>(mine, &t, misc);
+    tiles_all += t;
+  }
+  if (bad) atomicExch(&g_cache_attn_split_range, 1);
+  // No more CTAs than units take part, so each of them has one and every contributor arrives.
+  const int64_t U = tiles_all * hp, G = min((int64_t)gridDim.x, U);
+  if (blockIdx.x >= G) return;
+  int64_t u0 = blockIdx.x * U / G, u1 = (blockIdx.x + 1) * U / G;
+  if (a.B <= L::THREADS) {
+    if (mine && u0 >= before * hp && u0 < (before + (int64_t)mine) * hp) {
+      misc[16] = threadIdx.x;
+      misc[17] = before;
+    }
+  } else {
+    int64_t run = 0;
+    for (int b0 = 0; b0 < a.B; b0 += L::THREADS) {
+      const int b = b0 + threadIdx.x;
+      bool bb;
+      const int n = b < a.B ? cs_seq(a, b, &bb).tiles : 0;
+      int t;
+      const int64_t at = run + block_scan<L::THREADS>(n, &t, misc);
+      run += t;
+      if (n && u0 >= at * hp && u0 < (at + n) * hp) {
+        misc[16] = b;
+        misc[17] = (int)at;
+      }
+    }
+  }
+  __syncthreads();
+  CsWalk walk;
+  walk.b = misc[16];
+  walk.before = misc[17];
+  walk.s = cs_seq(a, walk.b, &bad);
+  if (g.align_pairs) {
+    // whole pairs only: a range starts and ends at the next pair's first unit
+    CsWalk w = walk;
+    cs_seek(g, w, u0);
+    if (w.tile) u0 += w.s.tiles - w.tile;
+    if (u1 < U) {
+      cs_seek(g, w, u1);
+      if (w.tile) u1 += w.s.tiles - w.tile;
+    }
+    if (u0 >= u1) return;
+    cs_seek(g, walk, u0);
+  }
+  const int nun = (int)(u1 - u0);
+
+  if (warp == WARPS) {
+    // ------------------------------ producer ------------------------------
+    const int nch = CS_KEYS / g.chunk, per = 32 / nch; // chunks per tile, tiles per batch
+    const int my = lane / nch, ch = lane % nch;
+    const uint32_t chunk_bytes = (uint32_t)(g.chunk * 128 * 2 * NB);
+    if (lane == 0) {
+      tc::prefetch_tensormap(&map_k);
+      tc::prefetch_tensormap(&map_v);
+    }
+    bool stop = false;
+    int issued = 0;
+    for (int i0 = 0; i0 < nun && !stop; i0 += per) {
+      // this lane's chunk of tile i0 + my
+      bool valid = false;
+      int row = 0, z = 0;
+      float ks = 0.0f, vs = 0.0f;
+      if (i0 + my < nun) {
+        cs_seek(g, walk, u0 + i0 + my);
+        const int kvh = walk.pair / g.packs, pack = walk.pair % g.packs;
+        const int key0 = cs_key0(walk.s, walk.tile), j = key0 + ch * g.chunk;
+        int pf, pl;
+        cs_pack(g, walk.s, pack, RP, &pf, &pl);
+        if (cs_live(g, walk.s, pf, pl, key0) && j < walk.s.sp.total) {
+          const int page = j / a.T;
+          const int64_t id = a.table[(int64_t)walk.b * a.max_pages + page];
+          if (id >= 0 && id < a.pages) {
+            valid = true;
+            row = j - page * a.T;
+            z = (int)id * a.Hkv + kvh;
+            ks = a.ks[z];
+            vs = a.vs[z];
+          } else {
+            atomicExch(&g_cache_attn_split_range, 1);
+          }
+        }
+      }
+      const uint32_t have = __ballot_sync(0xffffffffu, valid);
+      auto copy = [&](int k) { // this lane's boxes of tile i0 + k
+        if (my == k && valid) {
+          const int s = (i0 + k) % STAGES;
+          uint8_t *st = sm + s * L::STAGE + ch * g.chunk * 128;
+#pragma unroll
+          for (int x = 0; x < NB; ++x) {
+            tc::tma_load_3d(st + x * CS_BOX, &map_k, &full[s], x * 128, row, z);
+            tc::tma_load_3d(st + (NB + x) * CS_BOX, &map_v, &full[s], x * 128, row, z);
+          }
+        }
+      };
+      const int n = min(per, nun - i0);
+      // The first fill of the ring: every copy starts before the first scale is waited for (a copy
+      // may land before its bytes are expected; the phase stays open until the arrival below).
+      const int early = i0 == 0 ? min(n, STAGES) : 0;
+      for (int k = 0; k < early; ++k) copy(k);
+      for (int k = 0; k < n; ++k) {
+        const int i = i0 + k, s = i % STAGES;
+        if (i >= STAGES) {
+          bool ok = !flags[0] && tc::mbar_wait(&empty[s], ((i / STAGES) - 1) & 1);
+          if (!__all_sync(0xffffffffu, ok)) {
+            if (lane == 0) {
+              atomicExch(&g_cache_attn_split_status, tc::kTimeoutEmpty);
+              flags[0] = 1;
+            }
+            stop = true;
+            break;
+          }
+        }
+        if (my == k) // key scale in score units; value scale; its logarithm; validity
+          sc[s * 4 + ch] = make_float4(ks * a.scale * kLog2E, vs, fminf(fmaxf(log2f(vs), -60.0f), 110.0f),
+                                       valid ? 1.0f : 0.0f);
+        __syncwarp();
+        if (lane == 0) {
+          const uint32_t mask = (nch == 32 ? 0xffffffffu : ((1u << nch) - 1u)) << (k * nch);
+          tc::mbar_expect_tx(&full[s], (uint32_t)__popc(have & mask) * chunk_bytes);
+        }
+        __syncwarp();
+        if (k >= early) copy(k);
+        issued = i + 1;
+      }
+    }
+    // After a give-up no copy may land once the CTA has left: wait (bounded) for the last fills.
+    if (stop)
+      for (int i = max(0, issued - STAGES); i < issued; ++i) tc::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+    return;
+  }
+
+  // ------------------------------ consumers -------------------------------
+  const int gq = lane >> 2, t = lane & 3;
+  bool ok = true;
+  int64_t first_pair = -1; // global number of the range's first pair
+  int seg0 = 0;
+  while (seg0 < nun) {
+    cs_seek(g, walk, u0 + seg0);
+    const CsSeq seq = walk.s;
+    const int seg1 = min(nun, seg0 + seq.tiles - walk.tile);
+    const int kvh = walk.pair / g.packs, pack = walk.pair % g.packs;
+    const int64_t pair = (int64_t)walk.b * hp + walk.pair;
+    if (first_pair < 0) first_pair = pair;
+    const int rows = min(RP, g.rows - pack * RP);
+    int pos_first, pos_last;
+    cs_pack(g, seq, pack, RP, &pos_first, &pos_last);
+
+    // ---- queries: B fragments, lane (gq, t) holds row gq of each 8-row tile ----
+    // k step s of box x covers columns 128 x + 32 t + 4 s .. + 3 of lane t (16 t + 4 s when DP is 64).
+    uint32_t qb[NT][KS][2];
+    float qf[NT][2]; // power of two of the columns' rows 2t, 2t + 1
+    int hi[NT][2], lo[NT][2]; // last key seen, first key of the window
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = pack * RP + nt * 8 + gq;
+      const bool in = r < g.rows;
+      const T *qp = static_cast<const T *>(a.q) + (int64_t)walk.b * a.q_b +
+                    (in ? (int64_t)(kvh * a.group + r % a.group) * a.q_h + (int64_t)(r / a.group) * a.q_s : 0);
+      constexpr int COLS = DP == 64 ? 16 : 32;
+      float f = 1.0f;
+#pragma unroll
+      for (int x = 0; x < NB; ++x)
+#pragma unroll
+        for (int c = 0; c < COLS / 8; ++c) {
+          const int d = x * 128 + COLS * t + 8 * c;
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (in && d < a.D) v = *reinterpret_cast<const uint4 *>(qp + d); // D is a multiple of 16
+          const int k = x * 8 + 2 * c;
+          qb[nt][k][0] = v.x;
+          qb[nt][k][1] = v.y;
+          qb[nt][k + 1][0] = v.z;
+          qb[nt][k + 1][1] = v.w;
+        }
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        // the row's largest exponent, over the four lanes of the row
+        uint32_t e = 0u;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) e = max(e, max(qb[nt][k][i] & 0x7f80u, (qb[nt][k][i] >> 16) & 0x7f80u));
+        e = max(e, __shfl_xor_sync(0xffffffffu, e, 1));
+        e = max(e, __shfl_xor_sync(0xffffffffu, e, 2));
+        const int ex = min(max((int)(e >> 7) - 127, -126), 126);
+        const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
+        f = __uint_as_float((uint32_t)(127 + ex) << 23);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            qb[nt][k][i] = half2_of(__uint_as_float(qb[nt][k][i] << 16) * down,
+                                    __uint_as_float(qb[nt][k][i] & 0xffff0000u) * down);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        qf[nt][e] = __shfl_sync(0xffffffffu, f, (2 * t + e) * 4);
+        const int rc = pack * RP + nt * 8 + 2 * t + e, i = rc / a.group, p = seq.sp.past + i;
+        const bool counts = rc < g.rows && i < seq.sp.count;
+        hi[nt][e] = !counts ? -1 : a.causal ? min(p, seq.sp.total - 1) : seq.sp.total - 1;
+        lo[nt][e] = a.causal && a.window >= 0 ? p - a.window : 0;
+      }
+    }
+    float o[NT][KS][4]; // [columns 16 gq + 2 i (+1)][rows 2t, 2t + 1]; 8 gq + 2 i when DP is 64
+    float m_run[NT][2], l_run[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][k][e] = 0.0f;
+      m_run[nt][0] = m_run[nt][1] = -INFINITY;
+      l_run[nt][0] = l_run[nt][1] = 0.0f;
+    }
+
+    // A stage is always the same warp's, which frees its last fill before it waits for the next, so
+    // a parity wait cannot be satisfied by the fill before last.
+    for (int i = seg0 + ((warp - seg0 % WARPS + WARPS) % WARPS); i < seg1; i += WARPS) {
+      const int s = i % STAGES;
+      if (ok && flags[0]) ok = false;
+      if (ok && !tc::mbar_wait(&full[s], (i / STAGES) & 1)) {
+        atomicExch(&g_cache_attn_split_status, tc::kTimeoutFull);
+        flags[0] = 1;
+        ok = false;
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      const int key0 = cs_key0(seq, walk.tile + (i - seg0));
+      if (ok && cs_live(g, seq, pos_first, pos_last, key0)) {
+        const uint32_t kb = tc::smem_u32(sm + s * L::STAGE), vb = kb + NB * CS_BOX;
+        // scales of the tokens of this lane's S rows: gq and gq + 8 of each 16
+        float4 c4[2][2];
+        bool all = true;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            c4[mt][h] = sc[s * 4 + (mt * 16 + h * 8 + gq) / g.chunk];
+            all = all && c4[mt][h].w != 0.0f;
+          }
+        all = __all_sync(0xffffffffu, all);
+        const bool whole = all && key0 + CS_KEYS <= seq.sp.total;
+        if (!whole) {
+          // rows that hold no token of this sequence: their V codes must not reach the MMA
+#pragma unroll 1
+          for (int r = lane >> 3; r < CS_KEYS; r += 4) {
+            if (key0 + r >= seq.sp.total || sc[s * 4 + r / g.chunk].w == 0.0f)
+#pragma unroll
+              for (int x = 0; x < NB; ++x)
+                *reinterpret_cast<uint4 *>(sm + s * L::STAGE + (NB + x) * CS_BOX + r * 128 + (lane & 7) * 16) =
+                    make_uint4(0u, 0u, 0u, 0u);
+          }
+          tc::fence_proxy_async(); // before the stage's next TMA fill
+          __syncwarp();
+        }
+        const bool need_mask =
+            !whole || (a.causal && (key0 + CS_KEYS - 1 > pos_first ||
+                                    (a.window >= 0 && key0 < pos_last - a.window && key0 + CS_KEYS > a.sinks))) ||
+            pos_last - seq.sp.past != (pack * RP + rows - 1) / a.group; // rows that do not count
+        // ---- S^T = K . Q^T ----
+        float sv[2][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sv[mt][nt][e] = 0.0f;
+          const int r0 = mt * 16 + gq, r1 = r0 + 8;
+#pragma unroll
+          for (int x = 0; x < NB; ++x)
+#pragma unroll
+            for (int h = 0; h < (DP == 64 ? 1 : 2); ++h) {
+              const int u = DP == 64 ? t : 2 * t + h;
+              const uint4 k0 = lds128(unit_at(kb + x * CS_BOX, r0, u));
+              const uint4 k1 = lds128(unit_at(kb + x * CS_BOX, r1, u));
+              const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                uint32_t a0, a1, a2, a3;
+                to_half<Q>(w0[q], a0, a2);
+                to_half<Q>(w1[q], a1, a3);
+                const int k = x * 8 + h * 4 + q;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                  mma16816(sv[mt][nt], a0, a1, a2, a3, qb[nt][k][0], qb[nt][k][1]);
+              }
+            }
+        }
+        // ---- scores in base 2, masks, the running reference ----
+        float mx[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float4 c = c4[mt][e >> 1];
+              float v = sv[mt][nt][e] * qf[nt][e & 1] * c.x;
+              if (a.softcap > 0.0f) v = a.softcap * tanhf(v * kLn2 / a.softcap) * kLog2E;
+              if (need_mask) {
+                const int j = key0 + mt * 16 + (e >> 1) * 8 + gq;
+                const bool seen = j <= hi[nt][e & 1] && (j >= lo[nt][e & 1] || j < a.sinks) && c.w != 0.0f;
+                if (!seen) v = -INFINITY;
+              }
+              sv[mt][nt][e] = v;
+              mx[nt][e & 1] = fmaxf(mx[nt][e & 1], v + c.z);
+            }
+        float corr[NT][2], ref[NT][2];
+        bool moved = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) mx[nt][e] = fmaxf(mx[nt][e], __shfl_xor_sync(0xffffffffu, mx[nt][e], w));
+            const float mn = fmaxf(m_run[nt][e], mx[nt][e]);
+            const float base = mn == -INFINITY ? 0.0f : mn;
+            corr[nt][e] = exp2f(m_run[nt][e] - base);
+            ref[nt][e] = base - CS_LIFT;
+            moved = moved || mn != m_run[nt][e];
+            m_run[nt][e] = mn;
+          }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            l_run[nt][0] *= corr[nt][0];
+            l_run[nt][1] *= corr[nt][1];
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nt][k][e] *= corr[nt][e & 1];
+          }
+        }
+        // ---- P^T fragments ----
+        uint32_t pb[2][NT][2];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float v = sv[mt][nt][e];
+              p[e] = exp2f(v - ref[nt][e & 1]);
+              l_run[nt][e & 1] += p[e];
+              // a key that is not seen has p = 0 whatever its page's scale is
+              p[e] = v == -INFINITY ? 0.0f : p[e] * c4[mt][e >> 1].y;
+            }
+            pb[mt][nt][0] = transpose8(half2_of(p[0], p[1]));
+            pb[mt][nt][1] = transpose8(half2_of(p[2], p[3]));
+          }
+        // ---- O^T += V^T . P^T ----
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          const int r = mt * 16 + 2 * t;
+#pragma unroll
+          for (int x = 0; x < NB; ++x) {
+            uint32_t w[4][4]; // [token 2t, 2t + 1, 2t + 8, 2t + 9][4 columns each]
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int rr = r + (q & 1) + (q >> 1) * 8;
+              if constexpr (DP == 64) {
+                const uint2 v = lds64(unit_at(vb, rr, gq >> 1) + (gq & 1) * 8);
+                w[q][0] = v.x;
+                w[q][1] = v.y;
+              } else {
+                const uint4 v = lds128(unit_at(vb + x * CS_BOX, rr, gq));
+                w[q][0] = v.x;
+                w[q][1] = v.y;
+                w[q][2] = v.z;
+                w[q][3] = v.w;
+              }
+            }
+#pragma unroll
+            for (int c = 0; c < (DP == 64 ? 2 : 4); ++c) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) { // columns 4c + 2h, 4c + 2h + 1
+                const uint32_t sel = h ? 0x7362u : 0x5140u;
+                uint32_t a0, a1, a2, a3;
+                to_half<Q>(__byte_perm(w[0][c], w[1][c], sel), a0, a1);
+                to_half<Q>(__byte_perm(w[2][c], w[3][c], sel), a2, a3);
+                const int k = x * 8 + 2 * c + h;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][k], a0, a1, a2, a3, pb[mt][nt][0], pb[mt][nt][1]);
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&empty[s]);
+    }
+
+    // ---------------- end of a pair's segment: merge the warps ----------------
+    auto consumers_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); };
+    consumers_sync(); // the merge buffer is free
+    constexpr int W = DP + 2;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l_run[nt][e] += __shfl_xor_sync(0xffffffffu, l_run[nt][e], 4);
+        l_run[nt][e] += __shfl_xor_sync(0xffffffffu, l_run[nt][e], 8);
+        l_run[nt][e] += __shfl_xor_sync(0xffffffffu, l_run[nt][e], 16);
+        float *mw = mrg + (size_t)(warp * RP + nt * 8 + 2 * t + e) * W;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const int d = DP == 64 ? 8 * gq + 2 * k : (k >> 3) * 128 + 16 * gq + 2 * (k & 7);
+          *reinterpret_cast<float2 *>(mw + d) = make_float2(o[nt][k][e], o[nt][k][2 + e]);
+        }
+        if (gq == 0) {
+          mw[DP] = m_run[nt][e];
+          mw[DP + 1] = l_run[nt][e];
+        }
+      }
+    consumers_sync();
+    // the pair's units, and the CTAs that hold some of them
+    const int64_t pu = walk.before * hp + (int64_t)walk.pair * seq.tiles;
+    const int64_t cf = ((pu + 1) * G - 1) / U, cl = ((pu + seq.tiles) * G - 1) / U;
+    const bool one = g.align_pairs || cf == cl;
+    float *part = g.partials + (((size_t)blockIdx.x * 2 + (pair == first_pair ? 0 : 1)) * RP) * W;
+    auto put = [&](int r, int d, float acc, float l) {
+      const int rr = pack * RP + r;
+      st1<T>(a.y, (int64_t)walk.b * a.q_b + (int64_t)(kvh * a.group + rr % a.group) * a.q_h +
+                      (int64_t)(rr / a.group) * a.q_s + d,
+             l == 0.0f ? 0.0f : acc / l);
+    };
+    for (int e = threadIdx.x; e < rows * DP; e += WARPS * 32) {
+      const int r = e / DP, d = e % DP;
+      if (d >= a.D) continue;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, mrg[(size_t)(w * RP + r) * W + DP]);
+      const float base = M == -INFINITY ? 0.0f : M;
+      float l = 0.0f, acc = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float *row = mrg + (size_t)(w * RP + r) * W;
+        const float c = exp2f(row[DP] - base);
+        l += row[DP + 1] * c;
+        acc += row[d] * c;
+      }
+      if (one) {
+        if (ok) put(r, d, acc, l);
+      } else {
+        part[r * W + d] = acc;
+        if (d == 0) {
+          part[r * W + DP] = M;
+          part[r * W + DP + 1] = l;
+        }
+      }
+    }
+    if (!one) {
+      consumers_sync();
+      if (threadIdx.x == 0) {
+        const uint32_t inc = flags[0] ? kAbortMark + 1u : 1u;
+        const uint32_t now = arrive_acq_rel(g.counters + pair, inc) + inc;
+        const bool last = (now & (kAbortMark - 1u)) == (uint32_t)(cl - cf + 1);
+        if (last) g.counters[pair] = 0u;
+        flags[1] = last && (now >> 16) == 0u ? 1 : 0;
+      }
+      consumers_sync();
+      if (flags[1] && ok) {
+        // the last CTA of this pair: the partials in CTA order.  Only cf can hold the pair in its
+        // second slot: every later CTA's range starts inside it.
+        const int slot = cf * U / G < pu ? 1 : 0;
+        for (int e = threadIdx.x; e < rows * DP; e += WARPS * 32) {
+          const int r = e / DP, d = e % DP;
+          if (d >= a.D) continue;
+          float M = -INFINITY;
+          for (int64_t c = cf; c <= cl; ++c)
+            M = fmaxf(M, __ldcg(g.partials + ((c * 2 + (c == cf ? slot : 0)) * RP + r) * W + DP));
+          const float base = M == -INFINITY ? 0.0f : M;
+          float l = 0.0f, acc = 0.0f;
+          for (int64_t c = cf; c <= cl; ++c) {
+            const float *row = g.partials + ((c * 2 + (c == cf ? slot : 0)) * RP + r) * W;
+            const float w = exp2f(__ldcg(row + DP) - base);
+            l += __ldcg(row + DP + 1) * w;
+            acc += __ldcg(row + d) * w;
+          }
+          put(r, d, acc, l);
+        }
+      }
+    }
+    seg0 = seg1;
+  }
+}
+
+// Rows of a pack in eights: as few as hold all rows, up to 32 (16 for heads above 128, whose
+// accumulators fill the registers).
+int cs_nt(int64_t rows, int dp) { return rows <= 8 ? 1 : rows <= 16 || dp == 256 ? 2 : 4; }
+
+template <typename T, typename Q, int DP, int NT>
+int cs_launch(const CUtensorMap &mk, const CUtensorMap &mv, const CsArgs &g, unsigned grid, cudaStream_t st) {
+  using L = CsLayout<DP, NT>;
+  auto kern = cache_attn_split<T, Q, DP, NT>;
+  B2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::SMEM));
+  kern<<<grid, L::THREADS, L::SMEM, st>>>(mk, mv, g);
+  B2_LAUNCH_CHECK();
+  return B2_OK;
+}
+
+template <typename T, typename Q>
+int cs_pick(int dp, int nt, const CUtensorMap &mk, const CUtensorMap &mv, const CsArgs &g, unsigned grid,
+            cudaStream_t st) {
+  if (dp == 64) {
+    if (nt == 1) return cs_launch<T, Q, 64, 1>(mk, mv, g, grid, st);
+    if (nt == 2) return cs_launch<T, Q, 64, 2>(mk, mv, g, grid, st);
+    return cs_launch<T, Q, 64, 4>(mk, mv, g, grid, st);
+  }
+  if (dp == 128) {
+    if (nt == 1) return cs_launch<T, Q, 128, 1>(mk, mv, g, grid, st);
+    if (nt == 2) return cs_launch<T, Q, 128, 2>(mk, mv, g, grid, st);
+    return cs_launch<T, Q, 128, 4>(mk, mv, g, grid, st);
+  }
+  if (nt == 1) return cs_launch<T, Q, 256, 1>(mk, mv, g, grid, st);
+  return cs_launch<T, Q, 256, 2>(mk, mv, g, grid, st);
+}
+
+int dp_of(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
+} // namespace
+
+// Head sizes that are multiples of 16 up to 256, pages that are multiples of 8 tokens, 16-byte
+// aligned Q and cache (TMA), and counts that fit 32 bits.
+bool cache_attn_split_eligible(const CaArgs &a) {
+  const int64_t rows = (int64_t)a.S * a.group, nt = cs_nt(rows, dp_of(a.D));
+  const int64_t packs = (rows + 8 * nt - 1) / (8 * nt);
+  const int64_t tiles = (int64_t)a.max_pages * a.T / CS_KEYS + 2;
+  return a.D % 16 == 0 && a.D <= 256 && a.T % 8 == 0 && aligned(a.q, 16) && aligned(a.k, 16) &&
+         aligned(a.v, 16) && a.pages > 0 && rows < ((int64_t)1 << 30) &&
+         (double)a.B * a.Hkv * packs * tiles < 1e9;
+}
+
+size_t cache_attn_split_workspace(const CaArgs &a) {
+  const int dp = dp_of(a.D), nt = cs_nt((int64_t)a.S * a.group, dp);
+  return kCounterBytes + (size_t)sm_count() * 2 * 8 * nt * (dp + 2) * 4;
+}
+
+int cache_attn_split_launch(const CaArgs &a, bool f16, bool f8, void *ws, cudaStream_t st) {
+  const int dp = dp_of(a.D), nt = cs_nt((int64_t)a.S * a.group, dp);
+  CsArgs g{};
+  g.c = a;
+  g.rows = a.S * a.group;
+  g.packs = (g.rows + 8 * nt - 1) / (8 * nt);
+  g.chunk = a.T % 32 == 0 ? 32 : a.T % 16 == 0 ? 16 : 8;
+  g.align_pairs = (int64_t)a.B * a.Hkv * g.packs > (int64_t)kMaxCounters;
+  g.counters = static_cast<uint32_t *>(ws);
+  g.partials = reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + kCounterBytes);
+  // [pages * Hkv][T][D] codes; columns past D read as zeros
+  CUtensorMap mk, mv;
+  const uint64_t dims[3] = {(uint64_t)a.D, (uint64_t)a.T, (uint64_t)a.pages * a.Hkv};
+  const uint64_t strides[2] = {(uint64_t)a.D, (uint64_t)a.T * a.D};
+  const uint32_t box[3] = {128, (uint32_t)g.chunk, 1};
+  if (int rc = make_tensor_map(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  if (int rc = make_tensor_map(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  const unsigned grid = (unsigned)sm_count();
+  if (f16) return f8 ? cs_pick<__half, Fp8>(dp, nt, mk, mv, g, grid, st) : cs_pick<__half, Int8>(dp, nt, mk, mv, g, grid, st);
+  return f8 ? cs_pick<__nv_bfloat16, Fp8>(dp, nt, mk, mv, g, grid, st)
+            : cs_pick<__nv_bfloat16, Int8>(dp, nt, mk, mv, g, grid, st);
+}
+
+namespace {
+int read_word(int reset, const int &symbol) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, symbol, sizeof(int)) != cudaSuccess) return -1;
+  if (reset && v) {
+    const int z = 0;
+    if (cudaMemcpyToSymbol(symbol, &z, sizeof(int)) != cudaSuccess) return -1;
+  }
+  return v;
+}
+} // namespace
+int status_read_cache_attn_split(int reset) { return read_word(reset, g_cache_attn_split_status); }
+int range_read_cache_attn_split(int reset) { return read_word(reset, g_cache_attn_split_range); }
+
+} // namespace b2

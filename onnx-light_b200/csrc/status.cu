@@ -31,6 +31,8 @@ int status_read_gemv_n(int reset);
 int status_read_gemv_c(int reset);
 int status_read_cache_append(int reset);
 int status_read_cache_attention(int reset);
+int status_read_cache_attn_split(int reset);
+int range_read_cache_attn_split(int reset);
 
 __device__ int g_selftest_status;
 
@@ -73,7 +75,9 @@ extern "C" B2_API int b2_kernel_status(int reset) {
                       {"allgather_cols", status_read_allgather, 0},
                       {"kernel::RotaryEmbedding", status_read_rotary, kOutOfRange},
                       {"b200::KVCacheAppend", status_read_cache_append, kCacheRange},
-                      {"b200::QuantizedCacheAttention", status_read_cache_attention, kCacheRange}};
+                      {"b200::QuantizedCacheAttention", status_read_cache_attention, kCacheRange},
+                      {"b200::QuantizedCacheAttention", range_read_cache_attn_split, kCacheRange},
+                      {"cache_attn_split", status_read_cache_attn_split, 0}};
   int first = 0;
   for (const Src &s : srcs) {
     const int v = s.read(reset);
