@@ -5,20 +5,12 @@
 //
 // This file: checks, the choice of the kernel, and scaled_mm_any, the CUDA-core kernel for shapes the
 // others do not take (64 x 64 tiles, 32 columns of K staged in shared memory, 4 x 4 sums a thread).
-#include "quant8.cuh"
+#include "scaled_matmul.cuh"
 
 namespace b2 {
 namespace {
 
 using namespace q8;
-
-struct SmArgs {
-  const uint8_t *a, *w;
-  const float *as, *ws;
-  void *y;
-  int64_t M, N, K;
-  int a_per_row, w_per_col; // scales per row / column (else one for all)
-};
 
 constexpr int SA_TILE = 64, SA_K = 32;
 
@@ -120,6 +112,8 @@ extern "C" int b2_scaled_matmul(const b2_tensor *a, const b2_tensor *a_scale, co
   g.w_per_col = nw == N && N > 1;
   const bool f8 = a->dtype == kF8E4M3FN;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (scaled_skinny_eligible(g)) return scaled_skinny_launch(g, y->dtype, f8, st);
+  if (scaled_tc_eligible(g)) return scaled_tc_launch(g, y->dtype, f8, st);
   if (y->dtype == kFloat16) return launch_any<__half>(g, f8, st);
   if (y->dtype == kBfloat16) return launch_any<__nv_bfloat16>(g, f8, st);
   return launch_any<float>(g, f8, st);

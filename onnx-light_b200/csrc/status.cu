@@ -31,6 +31,7 @@ int status_read_gemv_n(int reset);
 int status_read_gemv_c(int reset);
 int status_read_cache_append(int reset);
 int status_read_cache_attention(int reset);
+int status_read_scaled_tc(int reset);
 int status_read_cache_attn_split(int reset);
 int range_read_cache_attn_split(int reset);
 
@@ -77,7 +78,8 @@ extern "C" B2_API int b2_kernel_status(int reset) {
                       {"b200::KVCacheAppend", status_read_cache_append, kCacheRange},
                       {"b200::QuantizedCacheAttention", status_read_cache_attention, kCacheRange},
                       {"b200::QuantizedCacheAttention", range_read_cache_attn_split, kCacheRange},
-                      {"cache_attn_split", status_read_cache_attn_split, 0}};
+                      {"cache_attn_split", status_read_cache_attn_split, 0},
+                      {"scaled_mm_tc", status_read_scaled_tc, 0}};
   int first = 0;
   for (const Src &s : srcs) {
     const int v = s.read(reset);
