@@ -9,6 +9,7 @@ the reference kernel would throw (std::invalid_argument -> ValueError).
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 import threading
 
@@ -153,6 +154,27 @@ def lib() -> C.CDLL:
                 L.b2_dequantize_matmul_noalloc.argtypes = [T, T, T, T, C.c_int64, C.c_int32, T, P]
                 _lib = L
     return _lib
+
+
+_native = None
+
+
+def native():
+    """The module _b2torch (csrc/torch_binding.cpp), connected to the loaded library."""
+    global _native
+    if _native is None:
+        L = lib()
+        path = os.path.join(HERE, "_b2torch.so")
+        if not os.path.exists(path):
+            raise ImportError(f"{path} is missing: build it first (python onnx-light_b200/build.py).")
+        spec = importlib.util.spec_from_file_location("_b2torch", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.connect(check, *[C.cast(f, C.c_void_p).value for f in (
+            L.b2_rms_normalization_quantize, L.b2_scaled_matmul, L.b2_kv_cache_append,
+            L.b2_cache_attention)])
+        _native = mod
+    return _native
 
 
 def version() -> str:

@@ -2,7 +2,8 @@
 
 nvcc compiles each csrc/*.cu for `-gencode arch=compute_100a,code=sm_100a`
 (cross-compiles without a GPU) and links them into libonnxl_b200.so next to
-this file, with the CUDA runtime linked statically.
+this file, with the CUDA runtime linked statically.  csrc/torch_binding.cpp becomes the
+Python module _b2torch next to it (g++ against torch's headers).
 """
 from __future__ import annotations
 
@@ -16,6 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libonnxl_b200.so")
+BINDING = os.path.join(HERE, "_b2torch.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 FLAGS = [
@@ -48,6 +50,27 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _binding() -> None:
+    src = os.path.join(CSRC, "torch_binding.cpp")
+    if not _needs(BINDING, src):
+        return
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    includes = [os.path.join(root, "include"), os.path.join(root, "include/torch/csrc/api/include"),
+                os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-shared", "-fPIC", "-O2", "-std=c++17", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-isystem{i}" for i in includes], src, "-o", BINDING,
+           f"-L{os.path.join(root, 'lib')}", f"-L{os.path.join(cuda, 'lib64')}", "-ltorch_python",
+           "-ltorch_cpu", "-lc10", "-lc10_cuda", "-l:libcudart.so.12"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"building {BINDING} failed:\n{r.stdout}\n{r.stderr}")
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
@@ -59,6 +82,7 @@ def build(verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    _binding()
     return LIB
 
 

@@ -399,15 +399,6 @@ class SwiGLU:
 # ---------------------------------------------------------------------------
 
 
-def _new_codes(shape, dtype: int, device):
-    """An uninitialised tensor of 8-bit codes: torch.int8, or a QTensor of FLOAT8E4M3FN."""
-    if dtype == capi.INT8:
-        return torch.empty(shape, dtype=torch.int8, device=device)
-    if dtype == capi.FLOAT8E4M3FN:
-        return QTensor(torch.empty(shape, dtype=torch.uint8, device=device), dtype, tuple(shape))
-    raise ValueError("8-bit codes are INT8 or FLOAT8E4M3FN")
-
-
 @dataclass
 class QuantizedNorm:
     Y: object  # codes: torch.int8, or a QTensor of FLOAT8E4M3FN
@@ -432,24 +423,11 @@ class RMSNormalizationQuantize:
                  dtype: int = capi.FLOAT8E4M3FN, group_size: int = 0, out=None,
                  out_scale: Optional[torch.Tensor] = None,
                  out_sum: Optional[torch.Tensor] = None) -> QuantizedNorm:
-        shape = tuple(x.shape)
-        if out is None:
-            out = _new_codes(shape, dtype, x.device)
-        if out_scale is None:
-            if group_size < 0 or (group_size and shape[-1] % group_size):
-                raise ValueError("b200::RMSNormalizationQuantize: group_size must divide the number "
-                                 "of columns (0: one group per row).")
-            out_scale = torch.empty(shape[:-1] + (shape[-1] // group_size if group_size else 1,),
-                                    dtype=torch.float32, device=x.device)
-        if out_sum is None and residual is not None:
-            out_sum = torch.empty_like(x)
-        xd, sd, yd, ysd = _desc(x), _desc(scale), _desc(out), _desc(out_scale)
-        rd = _desc(residual) if residual is not None else None
-        hd = _desc(out_sum) if out_sum is not None else None
-        check(lib().b2_rms_normalization_quantize(xd.ref, _ref(rd), sd.ref, float(epsilon),
-                                                  int(group_size), yd.ref, ysd.ref, _ref(hd),
-                                                  stream_ptr(x.device)))
-        return QuantizedNorm(out, out_scale, out_sum)
+        y, y_scale, total = capi.native().rms_norm_quantize(
+            x, scale, residual, epsilon, dtype, group_size, out, out_scale, out_sum)
+        if out is None and dtype == capi.FLOAT8E4M3FN:
+            y = QTensor(y, dtype, tuple(y.shape))
+        return QuantizedNorm(y, y_scale, total)
 
 
 class ScaledMatMul:
@@ -464,14 +442,7 @@ class ScaledMatMul:
     def __call__(self, a, a_scale: torch.Tensor, w, w_scale: torch.Tensor,
                  dtype: torch.dtype = torch.float16,
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        if out is None:
-            out = torch.empty(tuple(a.shape[:-1]) + (int(w.shape[0]),), dtype=dtype,
-                              device=a.device)
-        ad, asd, wd, wsd, yd = _desc(a), _desc(a_scale), _desc(w), _desc(w_scale), _desc(out)
-        _call_with_workspace(lib().b2_scaled_matmul,
-                             (ad.ref, asd.ref, wd.ref, wsd.ref, yd.ref),
-                             (stream_ptr(out.device),), out.device)
-        return out
+        return capi.native().scaled_matmul(a, a_scale, w, w_scale, dtype, out)
 
 
 class QuantizedKVCache:
@@ -516,12 +487,6 @@ class QuantizedKVCache:
         """Counts the tokens of a finished step (an int, or INT32 [batch])."""
         self.lengths += new_lengths
 
-    def _descs(self):
-        """The struct of the C call and what keeps it alive."""
-        ds = [_desc(self.k, self.dtype), _desc(self.v, self.dtype), _desc(self.k_scale),
-              _desc(self.v_scale), _desc(self.block_table), _desc(self.lengths)]
-        return capi.B2QuantizedCache(*[C.pointer(d.t) for d in ds]), ds
-
 
 class KVCacheAppend:
     """Writes new keys and values behind the tokens a :class:`QuantizedKVCache` holds.
@@ -536,11 +501,7 @@ class KVCacheAppend:
 
     def __call__(self, K: torch.Tensor, V: torch.Tensor, cache: QuantizedKVCache,
                  new_lengths: Optional[torch.Tensor] = None) -> None:
-        kd, vd = _desc(K), _desc(V)
-        nd = _desc(new_lengths) if new_lengths is not None else None
-        cd, keep = cache._descs()
-        check(lib().b2_kv_cache_append(kd.ref, vd.ref, C.byref(cd), _ref(nd),
-                                       stream_ptr(K.device)))
+        capi.native().kv_cache_append(K, V, cache, new_lengths)
 
 
 @dataclass
@@ -570,16 +531,10 @@ class QuantizedCacheAttention:
                  attrs: Optional[CacheAttributes] = None,
                  new_lengths: Optional[torch.Tensor] = None,
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        attrs = attrs or CacheAttributes()
-        a = capi.B2CacheAttentionAttrs(int(attrs.has_scale), float(attrs.scale),
-                                       int(attrs.is_causal), float(attrs.softcap),
-                                       int(attrs.left_window_size), int(attrs.sink_tokens))
-        if out is None:
-            out = torch.empty_like(Q)
-        qd, yd = _desc(Q), _desc(out)
-        nd = _desc(new_lengths) if new_lengths is not None else None
-        cd, keep = cache._descs()
-        _call_with_workspace(lib().b2_cache_attention,
-                             (qd.ref, C.byref(cd), _ref(nd), C.byref(a), yd.ref),
-                             (stream_ptr(Q.device),), Q.device)
-        return out
+        a = attrs or _CAUSAL
+        return capi.native().cache_attention(Q, cache, new_lengths, out, a.has_scale, a.scale,
+                                             a.is_causal, a.softcap, a.left_window_size,
+                                             a.sink_tokens)
+
+
+_CAUSAL = CacheAttributes()
