@@ -48,13 +48,18 @@ constexpr int CS_KEYS = 32; // tokens per tile
 constexpr float CS_LIFT = 15.0f; // log2 of the largest p * v_scale
 constexpr uint32_t CS_BOX = CS_KEYS * 128; // one 128-byte-wide tile of codes
 constexpr size_t CS_SMEM_MAX = 232448;
+constexpr int CS_CTAS = 160; // at most, one per SM
 
 template <int DP, int NT> struct CsLayout {
   static constexpr int NB = DP == 256 ? 2 : 1;            // 128-byte boxes per row
-  static constexpr int WARPS = NT == 1 ? 8 : 4;           // consumers
+  // Consumer warps: 11 and the producer share the register file at 168 each, 7 at 255.
+  static constexpr int WARPS = NT == 1 && DP <= 128 ? 11 : DP <= 128 || NT == 1 ? 7 : 4;
   static constexpr int THREADS = (WARPS + 1) * 32;
   static constexpr uint32_t STAGE = 2 * NB * CS_BOX;      // K boxes, V boxes
-  static constexpr uint32_t MERGE = WARPS * 8 * NT * (DP + 2) * 4;
+  // the warps' (O, m, l); the last arriver of a pair keeps (m, weight) of each CTA and row there
+  static constexpr uint32_t MERGE = WARPS * 8 * NT * (DP + 2) * 4 > CS_CTAS * 8 * NT * 8
+                                        ? WARPS * 8 * NT * (DP + 2) * 4
+                                        : CS_CTAS * 8 * NT * 8;
   static constexpr uint32_t FIXED = 1024 + MERGE + 4096;  // alignment, merge, barriers, scales
   // Each stage belongs to one consumer warp (see the parity note in the kernel).
   static constexpr int STAGES = (int)((CS_SMEM_MAX - FIXED) / STAGE) / WARPS * WARPS < 24
@@ -65,7 +70,7 @@ template <int DP, int NT> struct CsLayout {
   static constexpr uint32_t OFF_SC = OFF_BAR + 24 * 16;   // float4 [STAGES][4]
   static constexpr uint32_t OFF_MISC = OFF_SC + 24 * 64;
   static constexpr size_t SMEM = OFF_MISC + 256 + 1024;
-  static_assert(STAGES >= WARPS && SMEM <= CS_SMEM_MAX, "shared memory");
+  static_assert(STAGES >= WARPS && STAGES >= 4 && SMEM <= CS_SMEM_MAX, "shared memory");
 };
 
 struct CsArgs {
@@ -298,86 +303,107 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
 
   if (warp == WARPS) {
     // ------------------------------ producer ------------------------------
-    const int nch = CS_KEYS / g.chunk, per = 32 / nch; // chunks per tile, tiles per batch
+    // Lane (my, ch) brings chunk ch of tile my of each batch of `per` tiles.  Page numbers are
+    // read two batches ahead and scales one, so no batch waits for them; within a batch, groups of
+    // up to 8 tiles go through the ring's protocol together, one tile a lane
+    // (at most half the ring, so that a group's stages are distinct and the others stay in flight).
+    const int nch = CS_KEYS / g.chunk, per = 32 / nch, grp = min(per, min(8, STAGES / 2));
     const int my = lane / nch, ch = lane % nch;
     const uint32_t chunk_bytes = (uint32_t)(g.chunk * 128 * 2 * NB);
     if (lane == 0) {
       tc::prefetch_tensormap(&map_k);
       tc::prefetch_tensormap(&map_v);
     }
-    bool stop = false;
-    int issued = 0;
-    for (int i0 = 0; i0 < nun && !stop; i0 += per) {
-      // this lane's chunk of tile i0 + my
-      bool valid = false;
-      int row = 0, z = 0;
-      float ks = 0.0f, vs = 0.0f;
-      if (i0 + my < nun) {
-        cs_seek(g, walk, u0 + i0 + my);
-        const int kvh = walk.pair / g.packs, pack = walk.pair % g.packs;
-        const int key0 = cs_key0(walk.s, walk.tile), j = key0 + ch * g.chunk;
+    struct Chunk {
+      int id, row, kvh; // page, row in the page
+      bool live;        // a key of it may be seen
+    };
+    // the page of this lane's chunk of tile i (of this CTA's)
+    auto find = [&](int i) {
+      Chunk c{0, 0, 0, false};
+      if (i < nun) {
+        cs_seek(g, walk, u0 + i);
+        const int pack = walk.pair % g.packs, key0 = cs_key0(walk.s, walk.tile), j = key0 + ch * g.chunk;
         int pf, pl;
         cs_pack(g, walk.s, pack, RP, &pf, &pl);
         if (cs_live(g, walk.s, pf, pl, key0) && j < walk.s.sp.total) {
           const int page = j / a.T;
-          const int64_t id = a.table[(int64_t)walk.b * a.max_pages + page];
-          if (id >= 0 && id < a.pages) {
-            valid = true;
-            row = j - page * a.T;
-            z = (int)id * a.Hkv + kvh;
-            ks = a.ks[z];
-            vs = a.vs[z];
-          } else {
-            atomicExch(&g_cache_attn_split_range, 1);
-          }
+          c.id = a.table[(int64_t)walk.b * a.max_pages + page];
+          c.row = j - page * a.T;
+          c.kvh = walk.pair / g.packs;
+          c.live = true;
         }
       }
-      const uint32_t have = __ballot_sync(0xffffffffu, valid);
-      auto copy = [&](int k) { // this lane's boxes of tile i0 + k
-        if (my == k && valid) {
-          const int s = (i0 + k) % STAGES;
-          uint8_t *st = sm + s * L::STAGE + ch * g.chunk * 128;
+      return c;
+    };
+    // its row of the pool in pages and heads, -1 when there is none; reports pages out of range
+    auto place = [&](const Chunk &c) {
+      if (!c.live) return -1;
+      if (c.id >= 0 && c.id < a.pages) return c.id * a.Hkv + c.kvh;
+      atomicExch(&g_cache_attn_split_range, 1);
+      return -1;
+    };
+    bool stop = false;
+    int issued = 0;
+    Chunk c0 = find(my), c1 = find(per + my);
+    int z0 = place(c0);
+    float ks = z0 >= 0 ? a.ks[z0] : 0.0f, vs = z0 >= 0 ? a.vs[z0] : 0.0f;
+    for (int i0 = 0; i0 < nun && !stop; i0 += per) {
+      const int i = i0 + my, s = i % STAGES;
+      const uint32_t have = __ballot_sync(0xffffffffu, z0 >= 0);
+      auto copy = [&] { // this lane's boxes
+        uint8_t *st = sm + s * L::STAGE + ch * g.chunk * 128;
 #pragma unroll
-          for (int x = 0; x < NB; ++x) {
-            tc::tma_load_3d(st + x * CS_BOX, &map_k, &full[s], x * 128, row, z);
-            tc::tma_load_3d(st + (NB + x) * CS_BOX, &map_v, &full[s], x * 128, row, z);
-          }
+        for (int x = 0; x < NB; ++x) {
+          tc::tma_load_3d(st + x * CS_BOX, &map_k, &full[s], x * 128, c0.row, z0);
+          tc::tma_load_3d(st + (NB + x) * CS_BOX, &map_v, &full[s], x * 128, c0.row, z0);
         }
       };
-      const int n = min(per, nun - i0);
-      // The first fill of the ring: every copy starts before the first scale is waited for (a copy
-      // may land before its bytes are expected; the phase stays open until the arrival below).
-      const int early = i0 == 0 ? min(n, STAGES) : 0;
-      for (int k = 0; k < early; ++k) copy(k);
-      for (int k = 0; k < n; ++k) {
-        const int i = i0 + k, s = i % STAGES;
-        if (i >= STAGES) {
-          bool ok = !flags[0] && tc::mbar_wait(&empty[s], ((i / STAGES) - 1) & 1);
-          if (!__all_sync(0xffffffffu, ok)) {
-            if (lane == 0) {
-              atomicExch(&g_cache_attn_split_status, tc::kTimeoutEmpty);
-              flags[0] = 1;
-            }
-            stop = true;
-            break;
+      // The first fill of the ring: every copy starts before its scales are waited for (a copy may
+      // land before its bytes are expected; the phase stays open until the arrival below).
+      const bool early = i < STAGES;
+      if (early && z0 >= 0) copy();
+      // the next batch's scales, and the pages of the one after
+      const int z1 = place(c1);
+      const float ks1 = z1 >= 0 ? a.ks[z1] : 0.0f, vs1 = z1 >= 0 ? a.vs[z1] : 0.0f;
+      const Chunk c2 = find(i + 2 * per);
+      for (int k = 0; k < per && i0 + k < nun; k += grp) {
+        const bool act = my >= k && my < k + grp && i < nun;
+        bool ok = true;
+        if (act && i >= STAGES) ok = tc::mbar_wait(&empty[s], ((i / STAGES) - 1) & 1);
+        ok = ok && !flags[0]; // consumers that gave up free stages without reading them
+        if (!__all_sync(0xffffffffu, ok)) {
+          if (lane == 0) {
+            atomicExch(&g_cache_attn_split_status, tc::kTimeoutEmpty);
+            flags[0] = 1;
           }
+          // early copies that are not expected yet: the wait below has to see them land
+          if (early && i >= issued && i < nun && ch == 0)
+            tc::mbar_expect_tx(&full[s], (uint32_t)__popc(have >> lane & ((1u << nch) - 1u)) * chunk_bytes);
+          issued = max(issued, min(min(nun, STAGES), i0 + per));
+          __syncwarp();
+          stop = true;
+          break;
         }
-        if (my == k) // key scale in score units; value scale; its logarithm; validity
+        if (act) // key scale in score units; value scale; its logarithm; validity
           sc[s * 4 + ch] = make_float4(ks * a.scale * kLog2E, vs, fminf(fmaxf(log2f(vs), -60.0f), 110.0f),
-                                       valid ? 1.0f : 0.0f);
+                                       z0 >= 0 ? 1.0f : 0.0f);
         __syncwarp();
-        if (lane == 0) {
-          const uint32_t mask = (nch == 32 ? 0xffffffffu : ((1u << nch) - 1u)) << (k * nch);
-          tc::mbar_expect_tx(&full[s], (uint32_t)__popc(have & mask) * chunk_bytes);
-        }
+        if (act && ch == 0)
+          tc::mbar_expect_tx(&full[s], (uint32_t)__popc(have >> lane & ((1u << nch) - 1u)) * chunk_bytes);
         __syncwarp();
-        if (k >= early) copy(k);
-        issued = i + 1;
+        if (act && !early && z0 >= 0) copy();
+        issued = min(nun, i0 + k + grp);
       }
+      c0 = c1;
+      c1 = c2;
+      z0 = z1;
+      ks = ks1;
+      vs = vs1;
     }
-    // After a give-up no copy may land once the CTA has left: wait (bounded) for the last fills.
-    if (stop)
-      for (int i = max(0, issued - STAGES); i < issued; ++i) tc::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+    // No copy may land once the CTA has left: wait (bounded) for each stage's last fill.  They
+    // are done already unless a wait gave up.
+    for (int i = max(0, issued - STAGES); i < issued; ++i) tc::mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
     return;
   }
 
@@ -713,23 +739,55 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
       consumers_sync();
       if (flags[1] && ok) {
         // the last CTA of this pair: the partials in CTA order.  Only cf can hold the pair in its
-        // second slot: every later CTA's range starts inside it.
-        const int slot = cf * U / G < pu ? 1 : 0;
+        // second slot: every later CTA's range starts inside it.  The contributors' weights
+        // 2^(m_c - m) come first, into the merge buffer (its partials are consumed), so that the
+        // sums then read their terms several at a time.
+        const int nc = (int)(cl - cf + 1);
+        const float *base_p = g.partials + (cf * 2 * RP) * (int64_t)W;
+        const int64_t first_at = cf * U / G < pu ? (int64_t)RP * W : 0; // of cf's slot
+        for (int e = threadIdx.x; e < rows * nc; e += WARPS * 32) {
+          const int r = e / nc, c = e - r * nc;
+          const float2 ml = __ldcg(reinterpret_cast<const float2 *>(
+              base_p + (c ? (int64_t)c * 2 * RP * W : first_at) + r * W + DP));
+          mrg[2 * e] = ml.x;
+          mrg[2 * e + 1] = ml.y;
+        }
+        consumers_sync();
+        for (int r = warp; r < rows; r += WARPS) { // one warp a row: largest m, weights, 1 / l
+          float *ml = mrg + 2 * r * nc;
+          float M = -INFINITY;
+          for (int c = lane; c < nc; c += 32) M = fmaxf(M, ml[2 * c]);
+#pragma unroll
+          for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+          const float base = M == -INFINITY ? 0.0f : M;
+          float l = 0.0f;
+          for (int c = lane; c < nc; c += 32) {
+            const float w = exp2f(ml[2 * c] - base);
+            l += ml[2 * c + 1] * w;
+            ml[2 * c] = w;
+          }
+#pragma unroll
+          for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+          __syncwarp();
+          if (lane == 0) ml[1] = l;
+        }
+        consumers_sync();
         for (int e = threadIdx.x; e < rows * DP; e += WARPS * 32) {
           const int r = e / DP, d = e % DP;
           if (d >= a.D) continue;
-          float M = -INFINITY;
-          for (int64_t c = cf; c <= cl; ++c)
-            M = fmaxf(M, __ldcg(g.partials + ((c * 2 + (c == cf ? slot : 0)) * RP + r) * W + DP));
-          const float base = M == -INFINITY ? 0.0f : M;
-          float l = 0.0f, acc = 0.0f;
-          for (int64_t c = cf; c <= cl; ++c) {
-            const float *row = g.partials + ((c * 2 + (c == cf ? slot : 0)) * RP + r) * W;
-            const float w = exp2f(__ldcg(row + DP) - base);
-            l += __ldcg(row + DP + 1) * w;
-            acc += __ldcg(row + d) * w;
+          const float *ml = mrg + 2 * r * nc;
+          const float *src = base_p + r * W + d;
+          float acc = __ldcg(src + first_at) * ml[0];
+          int c = 1;
+          for (; c + 8 <= nc; c += 8) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = __ldcg(src + (int64_t)(c + k) * 2 * RP * W);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc = fmaf(v[k], ml[2 * (c + k)], acc);
           }
-          put(r, d, acc, l);
+          for (; c < nc; ++c) acc = fmaf(__ldcg(src + (int64_t)c * 2 * RP * W), ml[2 * c], acc);
+          put(r, d, acc, ml[1]);
         }
       }
     }
@@ -768,6 +826,7 @@ int cs_pick(int dp, int nt, const CUtensorMap &mk, const CUtensorMap &mv, const 
   return cs_launch<T, Q, 256, 2>(mk, mv, g, grid, st);
 }
 
+int cs_grid() { return std::min(sm_count(), CS_CTAS); }
 int dp_of(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 } // namespace
@@ -785,7 +844,7 @@ bool cache_attn_split_eligible(const CaArgs &a) {
 
 size_t cache_attn_split_workspace(const CaArgs &a) {
   const int dp = dp_of(a.D), nt = cs_nt((int64_t)a.S * a.group, dp);
-  return kCounterBytes + (size_t)sm_count() * 2 * 8 * nt * (dp + 2) * 4;
+  return kCounterBytes + (size_t)cs_grid() * 2 * 8 * nt * (dp + 2) * 4;
 }
 
 int cache_attn_split_launch(const CaArgs &a, bool f16, bool f8, void *ws, cudaStream_t st) {
@@ -805,7 +864,7 @@ int cache_attn_split_launch(const CaArgs &a, bool f16, bool f8, void *ws, cudaSt
   const uint32_t box[3] = {128, (uint32_t)g.chunk, 1};
   if (int rc = make_tensor_map(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   if (int rc = make_tensor_map(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
-  const unsigned grid = (unsigned)sm_count();
+  const unsigned grid = (unsigned)cs_grid();
   if (f16) return f8 ? cs_pick<__half, Fp8>(dp, nt, mk, mv, g, grid, st) : cs_pick<__half, Int8>(dp, nt, mk, mv, g, grid, st);
   return f8 ? cs_pick<__nv_bfloat16, Fp8>(dp, nt, mk, mv, g, grid, st)
             : cs_pick<__nv_bfloat16, Int8>(dp, nt, mk, mv, g, grid, st);
