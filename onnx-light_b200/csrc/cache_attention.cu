@@ -191,6 +191,7 @@ extern "C" int b2_cache_attention(const b2_tensor *q, const b2_quantized_cache *
   B2_ENFORCE(q->data && y->data, "%s: a tensor has no data.", op);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool f8 = cache->k->dtype == kF8E4M3FN;
+  B2_ENFORCE(!split || q8::aligned(workspace, 16), "%s: the workspace must be 16-byte aligned.", op);
   if (split) return cache_attn_split_launch(a, q->dtype == kFloat16, f8, workspace, st);
   const unsigned grid = (unsigned)((B * Hq * S + CAA_WARPS - 1) / CAA_WARPS);
   if (q->dtype == kFloat16) {

@@ -56,10 +56,8 @@ template <int DP, int NT> struct CsLayout {
   static constexpr int WARPS = NT == 1 && DP <= 128 ? 11 : DP <= 128 || NT == 1 ? 7 : 4;
   static constexpr int THREADS = (WARPS + 1) * 32;
   static constexpr uint32_t STAGE = 2 * NB * CS_BOX;      // K boxes, V boxes
-  // the warps' (O, m, l); the last arriver of a pair keeps (m, weight) of each CTA and row there
-  static constexpr uint32_t MERGE = WARPS * 8 * NT * (DP + 2) * 4 > CS_CTAS * 8 * NT * 8
-                                        ? WARPS * 8 * NT * (DP + 2) * 4
-                                        : CS_CTAS * 8 * NT * 8;
+  static constexpr int W = DP + 4;                        // a row's O, m, l (16-byte rows)
+  static constexpr uint32_t MERGE = WARPS * 8 * NT * W * 4;
   static constexpr uint32_t FIXED = 1024 + MERGE + 4096;  // alignment, merge, barriers, scales
   // Each stage belongs to one consumer warp (see the parity note in the kernel).
   static constexpr int STAGES = (int)((CS_SMEM_MAX - FIXED) / STAGE) / WARPS * WARPS < 24
@@ -78,7 +76,7 @@ struct CsArgs {
   int packs, rows;  // packs of 8 NT rows of a KV head's `rows` = S * group
   int chunk;        // tokens per TMA box: a power of two, 8 to 32, that divides the page
   int align_pairs;  // CTA ranges start at pair boundaries (more pairs than counters)
-  float *partials;  // [grid][2][8 NT][DP + 2]: O, m, l
+  float *partials;  // [grid][2][8 NT][DP + 4]: O, m, l
   uint32_t *counters;
 };
 
@@ -161,16 +159,16 @@ struct CsWalk {
   CsSeq s;
   int pair, tile; // of the unit: KV head * packs + pack, tile
 };
-__device__ __forceinline__ void cs_seek(const CsArgs &g, CsWalk &w, int64_t u) {
-  const int64_t hp = (int64_t)g.c.Hkv * g.packs;
+__device__ __forceinline__ void cs_seek(const CsArgs &g, CsWalk &w, int u) {
+  const int hp = g.c.Hkv * g.packs;
   bool bad;
-  while (u >= (w.before + (int64_t)w.s.tiles) * hp) {
+  while (u >= (w.before + w.s.tiles) * hp) { // all units together stay below 2^30
     w.before += w.s.tiles;
     w.s = cs_seq(g.c, ++w.b, &bad);
   }
-  const int64_t r = u - w.before * hp;
-  w.pair = (int)(r / w.s.tiles);
-  w.tile = (int)(r - (int64_t)w.pair * w.s.tiles);
+  const int r = u - w.before * hp;
+  w.pair = r / w.s.tiles;
+  w.tile = r - w.pair * w.s.tiles;
 }
 // Positions of the pack's first and last query (last < first: none counts).
 __device__ __forceinline__ void cs_pack(const CsArgs &g, const CsSeq &s, int pack, int rows_per_pack,
@@ -233,7 +231,7 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
   volatile int *flags = misc + 24;                       // [0] abort [1] last
   const CaArgs &a = g.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t hp = (int64_t)a.Hkv * g.packs;
+  const int hp = a.Hkv * g.packs; // pairs per sequence
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
@@ -246,8 +244,7 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
   }
   // ---- this CTA's range of units ----
   bool bad = false;
-  int64_t tiles_all = 0;
-  int mine = 0, before = 0;
+  int tiles_all = 0, mine = 0, before = 0; // all sequences'; with B <= THREADS, of sequence threadIdx.x
   for (int b0 = 0; b0 < a.B; b0 += L::THREADS) {
     const int b = b0 + threadIdx.x;
     bool bb = false;
@@ -259,26 +256,51 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
   }
   if (bad) atomicExch(&g_cache_attn_split_range, 1);
   // No more CTAs than units take part, so each of them has one and every contributor arrives.
-  const int64_t U = tiles_all * hp, G = min((int64_t)gridDim.x, U);
-  if (blockIdx.x >= G) return;
-  int64_t u0 = blockIdx.x * U / G, u1 = (blockIdx.x + 1) * U / G;
-  if (a.B <= L::THREADS) {
-    if (mine && u0 >= before * hp && u0 < (before + (int64_t)mine) * hp) {
-      misc[16] = threadIdx.x;
-      misc[17] = before;
+  const int U = tiles_all * hp, G = min((int)gridDim.x, U), cta = blockIdx.x;
+  if (cta >= G) return;
+  const int share = U / G, extra = U - share * G; // the first `extra` CTAs take one more
+  int u0 = cta * share + min(cta, extra), u1 = u0 + share + (cta < extra);
+  // With few pairs, CTAs of one pair each where that costs at most a quarter more units per CTA: a CTA
+  // on a boundary would do two pairs' work and merges one after the other (for 8 pairs of 129 tiles
+  // it finished at 21 us, the others at 8).
+  bool own_pair = false;
+  int own_first = 0, own_count = 0; // the pair's CTAs
+  if (a.B <= L::THREADS && a.B * hp <= G && !g.align_pairs) {
+    const int q0 = (U + G - 1) / G;
+    for (int q = q0; q <= q0 + max(1, q0 / 4) && !own_pair; ++q) {
+      const int parts = (mine + q - 1) / q;
+      int all;
+      const int at = block_scan<L::THREADS>(parts, &all, misc) * hp;
+      if (all * hp > G) continue;
+      own_pair = true;
+      if (cta >= all * hp) return;
+      if (mine && cta >= at && cta < at + parts * hp) {
+        misc[16] = threadIdx.x;
+        misc[17] = before;
+        misc[18] = at;
+        misc[19] = parts;
+      }
     }
-  } else {
-    int64_t run = 0;
-    for (int b0 = 0; b0 < a.B; b0 += L::THREADS) {
-      const int b = b0 + threadIdx.x;
-      bool bb;
-      const int n = b < a.B ? cs_seq(a, b, &bb).tiles : 0;
-      int t;
-      const int64_t at = run + block_scan<L::THREADS>(n, &t, misc);
-      run += t;
-      if (n && u0 >= at * hp && u0 < (at + n) * hp) {
-        misc[16] = b;
-        misc[17] = (int)at;
+  }
+  if (!own_pair) {
+    if (a.B <= L::THREADS) {
+      if (mine && u0 >= before * hp && u0 < (before + mine) * hp) {
+        misc[16] = threadIdx.x;
+        misc[17] = before;
+      }
+    } else {
+      int run = 0;
+      for (int b0 = 0; b0 < a.B; b0 += L::THREADS) {
+        const int b = b0 + threadIdx.x;
+        bool bb;
+        const int n = b < a.B ? cs_seq(a, b, &bb).tiles : 0;
+        int t;
+        const int at = run + block_scan<L::THREADS>(n, &t, misc);
+        run += t;
+        if (n && u0 >= at * hp && u0 < (at + n) * hp) {
+          misc[16] = b;
+          misc[17] = at;
+        }
       }
     }
   }
@@ -287,7 +309,14 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
   walk.b = misc[16];
   walk.before = misc[17];
   walk.s = cs_seq(a, walk.b, &bad);
-  if (g.align_pairs) {
+  if (own_pair) {
+    const int at = misc[18], parts = misc[19], pair = (cta - at) / parts, part = cta - at - pair * parts;
+    own_first = cta - part;
+    own_count = parts;
+    const int n = walk.s.tiles, first = walk.before * hp + pair * n, q = n / parts, x = n - q * parts;
+    u0 = first + part * q + min(part, x);
+    u1 = u0 + q + (part < x);
+  } else if (g.align_pairs) {
     // whole pairs only: a range starts and ends at the next pair's first unit
     CsWalk w = walk;
     cs_seek(g, w, u0);
@@ -299,7 +328,7 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
     if (u0 >= u1) return;
     cs_seek(g, walk, u0);
   }
-  const int nun = (int)(u1 - u0);
+  const int nun = u1 - u0;
 
   if (warp == WARPS) {
     // ------------------------------ producer ------------------------------
@@ -410,14 +439,14 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
   // ------------------------------ consumers -------------------------------
   const int gq = lane >> 2, t = lane & 3;
   bool ok = true;
-  int64_t first_pair = -1; // global number of the range's first pair
+  int first_pair = -1; // number of the range's first pair
   int seg0 = 0;
   while (seg0 < nun) {
     cs_seek(g, walk, u0 + seg0);
     const CsSeq seq = walk.s;
     const int seg1 = min(nun, seg0 + seq.tiles - walk.tile);
     const int kvh = walk.pair / g.packs, pack = walk.pair % g.packs;
-    const int64_t pair = (int64_t)walk.b * hp + walk.pair;
+    const int pair = walk.b * hp + walk.pair;
     if (first_pair < 0) first_pair = pair;
     const int rows = min(RP, g.rows - pack * RP);
     int pos_first, pos_last;
@@ -533,34 +562,53 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
                                     (a.window >= 0 && key0 < pos_last - a.window && key0 + CS_KEYS > a.sinks))) ||
             pos_last - seq.sp.past != (pack * RP + rows - 1) / a.group; // rows that do not count
         // ---- S^T = K . Q^T ----
-        float sv[2][NT][4];
+        // With one tile of rows, even and odd steps have sums of their own: four short chains of MMAs.
+        constexpr int CH = NT == 1 ? 2 : 1;
+        float sv[2][NT][4], sx[CH][2][NT][4];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
+        for (int c = 0; c < CH; ++c)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sv[mt][nt][e] = 0.0f;
-          const int r0 = mt * 16 + gq, r1 = r0 + 8;
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int x = 0; x < NB; ++x)
+              for (int e = 0; e < 4; ++e) sx[c][mt][nt][e] = 0.0f;
 #pragma unroll
-            for (int h = 0; h < (DP == 64 ? 1 : 2); ++h) {
-              const int u = DP == 64 ? t : 2 * t + h;
-              const uint4 k0 = lds128(unit_at(kb + x * CS_BOX, r0, u));
-              const uint4 k1 = lds128(unit_at(kb + x * CS_BOX, r1, u));
-              const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+        for (int x = 0; x < NB; ++x)
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
+          for (int h = 0; h < (DP == 64 ? 1 : 2); ++h) {
+            const int u = DP == 64 ? t : 2 * t + h;
+            uint32_t w[2][2][4];
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const uint4 v = lds128(unit_at(kb + x * CS_BOX, mt * 16 + r * 8 + gq, u));
+                w[mt][r][0] = v.x;
+                w[mt][r][1] = v.y;
+                w[mt][r][2] = v.z;
+                w[mt][r][3] = v.w;
+              }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int mt = 0; mt < 2; ++mt) {
                 uint32_t a0, a1, a2, a3;
-                to_half<Q>(w0[q], a0, a2);
-                to_half<Q>(w1[q], a1, a3);
+                to_half<Q>(w[mt][0][q], a0, a2);
+                to_half<Q>(w[mt][1][q], a1, a3);
                 const int k = x * 8 + h * 4 + q;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
-                  mma16816(sv[mt][nt], a0, a1, a2, a3, qb[nt][k][0], qb[nt][k][1]);
+                  mma16816(sx[q % CH][mt][nt], a0, a1, a2, a3, qb[nt][k][0], qb[nt][k][1]);
               }
-            }
-        }
+          }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              sv[mt][nt][e] = CH == 2 ? sx[0][mt][nt][e] + sx[CH - 1][mt][nt][e] : sx[0][mt][nt][e];
         // ---- scores in base 2, masks, the running reference ----
         float mx[NT][2];
 #pragma unroll
@@ -671,7 +719,7 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
     // ---------------- end of a pair's segment: merge the warps ----------------
     auto consumers_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); };
     consumers_sync(); // the merge buffer is free
-    constexpr int W = DP + 2;
+    constexpr int W = L::W;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -691,40 +739,66 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
         }
       }
     consumers_sync();
-    // the pair's units, and the CTAs that hold some of them
-    const int64_t pu = walk.before * hp + (int64_t)walk.pair * seq.tiles;
-    const int64_t cf = ((pu + 1) * G - 1) / U, cl = ((pu + seq.tiles) * G - 1) / U;
-    const bool one = g.align_pairs || cf == cl;
-    float *part = g.partials + (((size_t)blockIdx.x * 2 + (pair == first_pair ? 0 : 1)) * RP) * W;
-    auto put = [&](int r, int d, float acc, float l) {
-      const int rr = pack * RP + r;
-      st1<T>(a.y, (int64_t)walk.b * a.q_b + (int64_t)(kvh * a.group + rr % a.group) * a.q_h +
-                      (int64_t)(rr / a.group) * a.q_s + d,
-             l == 0.0f ? 0.0f : acc / l);
+    // the pair's units, and the CTAs cf .. cl that hold some of them
+    const int pu = walk.before * hp + walk.pair * seq.tiles;
+    auto cta_of = [&](int u) {
+      const int thr = extra * (share + 1);
+      return u < thr ? u / (share + 1) : extra + (u - thr) / share;
     };
-    for (int e = threadIdx.x; e < rows * DP; e += WARPS * 32) {
-      const int r = e / DP, d = e % DP;
+    const int cf = own_pair ? own_first : cta_of(pu);
+    const int cl = own_pair ? own_first + own_count - 1 : cta_of(pu + seq.tiles - 1);
+    const bool one = g.align_pairs || cf == cl;
+    // Only cf can hold the pair in its second slot: every later CTA's range starts inside it.
+    const int cf_slot = !own_pair && cf * share + min(cf, extra) < pu ? 1 : 0;
+    float *part = g.partials + ((size_t)cta * 2 + (pair == first_pair ? 0 : 1)) * RP * W;
+    auto put = [&](int r, int d, float4 v, float l) { // four columns of row r
+      const int rr = pack * RP + r;
+      T *y = static_cast<T *>(a.y) + (int64_t)walk.b * a.q_b + (int64_t)(kvh * a.group + rr % a.group) * a.q_h +
+             (int64_t)(rr / a.group) * a.q_s + d;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      uint2 w;
+      if constexpr (std::is_same<T, __half>::value) {
+        w.x = half2_of(v.x * inv, v.y * inv);
+        w.y = half2_of(v.z * inv, v.w * inv);
+      } else {
+        const __nv_bfloat162 b0 = __floats2bfloat162_rn(v.x * inv, v.y * inv);
+        const __nv_bfloat162 b1 = __floats2bfloat162_rn(v.z * inv, v.w * inv);
+        w.x = *reinterpret_cast<const uint32_t *>(&b0);
+        w.y = *reinterpret_cast<const uint32_t *>(&b1);
+      }
+      *reinterpret_cast<uint2 *>(y) = w;
+    };
+    auto add = [](float4 &acc, const float4 &v, float w) {
+      acc.x = fmaf(v.x, w, acc.x);
+      acc.y = fmaf(v.y, w, acc.y);
+      acc.z = fmaf(v.z, w, acc.z);
+      acc.w = fmaf(v.w, w, acc.w);
+    };
+    const int nw = min(WARPS, seg1 - seg0), w0 = seg0 % WARPS, n4 = rows * (DP / 4);
+    for (int e = threadIdx.x; e < n4; e += WARPS * 32) {
+      const int r = e / (DP / 4), d = e % (DP / 4) * 4;
       if (d >= a.D) continue;
       float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, mrg[(size_t)(w * RP + r) * W + DP]);
+      for (int k = 0; k < nw; ++k) {
+        const int w = w0 + k < WARPS ? w0 + k : w0 + k - WARPS;
+        M = fmaxf(M, mrg[(w * RP + r) * W + DP]);
+      }
       const float base = M == -INFINITY ? 0.0f : M;
-      float l = 0.0f, acc = 0.0f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float *row = mrg + (size_t)(w * RP + r) * W;
-        const float c = exp2f(row[DP] - base);
-        l += row[DP + 1] * c;
-        acc += row[d] * c;
+      float l = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int k = 0; k < nw; ++k) {
+        const int w = w0 + k < WARPS ? w0 + k : w0 + k - WARPS;
+        const float *row = mrg + (w * RP + r) * W;
+        const float2 ml = *reinterpret_cast<const float2 *>(row + DP);
+        const float c = exp2f(ml.x - base);
+        l = fmaf(ml.y, c, l);
+        add(acc, *reinterpret_cast<const float4 *>(row + d), c);
       }
       if (one) {
         if (ok) put(r, d, acc, l);
       } else {
-        part[r * W + d] = acc;
-        if (d == 0) {
-          part[r * W + DP] = M;
-          part[r * W + DP + 1] = l;
-        }
+        *reinterpret_cast<float4 *>(part + r * W + d) = acc;
+        if (d == 0) *reinterpret_cast<float2 *>(part + r * W + DP) = make_float2(M, l);
       }
     }
     if (!one) {
@@ -738,56 +812,69 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
       }
       consumers_sync();
       if (flags[1] && ok) {
-        // the last CTA of this pair: the partials in CTA order.  Only cf can hold the pair in its
-        // second slot: every later CTA's range starts inside it.  The contributors' weights
-        // 2^(m_c - m) come first, into the merge buffer (its partials are consumed), so that the
-        // sums then read their terms several at a time.
-        const int nc = (int)(cl - cf + 1);
-        const float *base_p = g.partials + (cf * 2 * RP) * (int64_t)W;
-        const int64_t first_at = cf * U / G < pu ? (int64_t)RP * W : 0; // of cf's slot
-        for (int e = threadIdx.x; e < rows * nc; e += WARPS * 32) {
-          const int r = e / nc, c = e - r * nc;
-          const float2 ml = __ldcg(reinterpret_cast<const float2 *>(
-              base_p + (c ? (int64_t)c * 2 * RP * W : first_at) + r * W + DP));
-          mrg[2 * e] = ml.x;
-          mrg[2 * e + 1] = ml.y;
-        }
-        consumers_sync();
-        for (int r = warp; r < rows; r += WARPS) { // one warp a row: largest m, weights, 1 / l
-          float *ml = mrg + 2 * r * nc;
-          float M = -INFINITY;
-          for (int c = lane; c < nc; c += 32) M = fmaxf(M, ml[2 * c]);
+        // The last CTA of this pair: the partials in CTA order.  With threads to spare, `teams` of
+        // them share the CTAs (every teams-th each) and are joined in order through the merge
+        // buffer; a thread has up to eight partials in flight.
+        const int nc = cl - cf + 1, teams = max(1, WARPS * 32 / n4);
+        for (int x = threadIdx.x; x < (teams > 1 ? n4 * teams : n4); x += WARPS * 32) {
+          const int team = teams > 1 ? x / n4 : 0, e = x - team * n4;
+          const int r = e / (DP / 4), d = e % (DP / 4) * 4;
+          float M = -INFINITY, l = 0.0f;
+          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int c = team; c < nc; c += 8 * teams) {
+            float2 ml[8];
+            float4 v[8];
 #pragma unroll
-          for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-          const float base = M == -INFINITY ? 0.0f : M;
-          float l = 0.0f;
-          for (int c = lane; c < nc; c += 32) {
-            const float w = exp2f(ml[2 * c] - base);
-            l += ml[2 * c + 1] * w;
-            ml[2 * c] = w;
+            for (int k = 0; k < 8; ++k) {
+              const int cc = c + k * teams;
+              ml[k] = make_float2(-INFINITY, 0.0f);
+              v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if (cc < nc) {
+                const float *row = g.partials + ((size_t)(cf + cc) * 2 + (cc ? 0 : cf_slot)) * RP * W + r * W;
+                ml[k] = __ldcg(reinterpret_cast<const float2 *>(row + DP));
+                if (d < a.D) v[k] = __ldcg(reinterpret_cast<const float4 *>(row + d));
+              }
+            }
+            float mn = M;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) mn = fmaxf(mn, ml[k].x);
+            const float base = mn == -INFINITY ? 0.0f : mn, keep = exp2f(M - base);
+            l *= keep;
+            acc.x *= keep;
+            acc.y *= keep;
+            acc.z *= keep;
+            acc.w *= keep;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float w = exp2f(ml[k].x - base);
+              l = fmaf(ml[k].y, w, l);
+              add(acc, v[k], w);
+            }
+            M = mn;
           }
-#pragma unroll
-          for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-          __syncwarp();
-          if (lane == 0) ml[1] = l;
-        }
-        consumers_sync();
-        for (int e = threadIdx.x; e < rows * DP; e += WARPS * 32) {
-          const int r = e / DP, d = e % DP;
-          if (d >= a.D) continue;
-          const float *ml = mrg + 2 * r * nc;
-          const float *src = base_p + r * W + d;
-          float acc = __ldcg(src + first_at) * ml[0];
-          int c = 1;
-          for (; c + 8 <= nc; c += 8) {
-            float v[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = __ldcg(src + (int64_t)(c + k) * 2 * RP * W);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) acc = fmaf(v[k], ml[2 * (c + k)], acc);
+          if (teams > 1) {
+            *reinterpret_cast<float4 *>(mrg + 8 * x) = acc;
+            *reinterpret_cast<float2 *>(mrg + 8 * x + 4) = make_float2(M, l);
+          } else if (d < a.D) {
+            put(r, d, acc, l);
           }
-          for (; c < nc; ++c) acc = fmaf(__ldcg(src + (int64_t)c * 2 * RP * W), ml[2 * c], acc);
-          put(r, d, acc, ml[1]);
+        }
+        if (teams > 1) {
+          consumers_sync();
+          for (int e = threadIdx.x; e < n4; e += WARPS * 32) {
+            const int r = e / (DP / 4), d = e % (DP / 4) * 4;
+            float M = -INFINITY, l = 0.0f;
+            for (int team = 0; team < teams; ++team) M = fmaxf(M, mrg[8 * (team * n4 + e) + 4]);
+            const float base = M == -INFINITY ? 0.0f : M;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int team = 0; team < teams; ++team) {
+              const float *p = mrg + 8 * (team * n4 + e);
+              const float w = exp2f(p[4] - base);
+              l = fmaf(p[5], w, l);
+              add(acc, *reinterpret_cast<const float4 *>(p), w);
+            }
+            if (d < a.D) put(r, d, acc, l);
+          }
         }
       }
     }
@@ -838,13 +925,13 @@ bool cache_attn_split_eligible(const CaArgs &a) {
   const int64_t packs = (rows + 8 * nt - 1) / (8 * nt);
   const int64_t tiles = (int64_t)a.max_pages * a.T / CS_KEYS + 2;
   return a.D % 16 == 0 && a.D <= 256 && a.T % 8 == 0 && aligned(a.q, 16) && aligned(a.k, 16) &&
-         aligned(a.v, 16) && a.pages > 0 && rows < ((int64_t)1 << 30) &&
+         aligned(a.v, 16) && aligned(a.y, 8) && a.pages > 0 && rows < ((int64_t)1 << 30) &&
          (double)a.B * a.Hkv * packs * tiles < 1e9;
 }
 
 size_t cache_attn_split_workspace(const CaArgs &a) {
   const int dp = dp_of(a.D), nt = cs_nt((int64_t)a.S * a.group, dp);
-  return kCounterBytes + (size_t)cs_grid() * 2 * 8 * nt * (dp + 2) * 4;
+  return kCounterBytes + (size_t)cs_grid() * 2 * 8 * nt * (dp + 4) * 4;
 }
 
 int cache_attn_split_launch(const CaArgs &a, bool f16, bool f8, void *ws, cudaStream_t st) {
