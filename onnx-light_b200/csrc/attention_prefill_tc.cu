@@ -42,6 +42,7 @@
 // skips the rest, frees its TMEM and exits.
 #include <type_traits>
 
+#include "attn_math.cuh"
 #include "b2_common.cuh"
 #include "tc_common.cuh"
 
@@ -119,48 +120,6 @@ __device__ __forceinline__ void load_scores(const uint32_t (&r)[32], float (&v)[
       if (key >= g.L || (g.causal && key > pos)) v[off + e] = -INFINITY;
     }
   }
-}
-
-// 2^x with the hardware approximation (relative error about 2^-22; inputs are
-// <= 8 here, and -inf gives 0).
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Three-way maximum (one instruction on sm_100).
-__device__ __forceinline__ float max3f(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-// Element-wise a * b + c, a + b and a - b on two fp32 lanes (one packed
-// instruction each on sm_100; the same IEEE operation per element).
-__device__ __forceinline__ uint64_t f2pack(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ float2 f2unpack(uint64_t r) {
-  float2 v;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
-  return v;
-}
-__device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t fsub2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
 }
 
 template <typename T>

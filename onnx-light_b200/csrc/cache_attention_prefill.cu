@@ -1,0 +1,617 @@
+// Attention of prompts over a paged 8-bit KV cache (b2_cache_attention) on tcgen05 tensor cores:
+// FLOAT16 / BFLOAT16 queries, head sizes that are multiples of 16 up to 128, pages of whole 16s.
+//
+// Bound: tensor pipe and the exponentials, one of each per score.
+//
+// One CTA owns 128 query rows -- pk heads of one GQA group (pk the largest power of two up to 8 that
+// divides the group) x 128 / pk positions -- and walks the 128-key tiles that any of them sees (the
+// sinks' tiles, then the window's up to the diagonal):
+//   warps 9-11 (converters) read the tile's codes from their pages, 16 bytes a lane, widen them to
+//              FLOAT16 (exact for both code types) and write the 128-byte-swizzled K and V
+//              operands, two buffers each; rows that hold no token become zeros;
+//   warp 8     (MMA) issues S = Q K^T into one of two TMEM buffers and O += P V with P read from TMEM;
+//   warps 0-7  (softmax) two threads per query row, one per half of the columns.
+// Scales never touch an element: within 16 keys of one page the key scale is part of the exponent's
+// factor and log2 of the value scale part of its offset, p' = 2^(s k_scale + log2 v_scale - m), so O
+// sums p' code and the denominator sums p' / v_scale, one multiplication per 16 keys.  m follows
+// the row's largest exponent lazily: it is moved only when p' would pass 2^15, then to 2^7, and O
+// and l are rescaled; p' in FLOAT16 keeps 11 bits down to 2^-21 of the row's largest and more.
+// BFLOAT16 queries become FLOAT16 after a power of two per row (8 significant bits fit in 11).
+//
+// Every mbarrier is waited phase by phase by the threads that depend on it, and no barrier can run
+// two phases ahead of a waiter.  All waits are bounded; after a time-out the CTA records a code,
+// waits for its MMAs in flight, frees its TMEM and returns.
+#include <type_traits>
+
+#include "attn_math.cuh"
+#include "cache_attention.cuh"
+#include "tc_common.cuh"
+
+namespace b2 {
+
+__device__ int g_cache_attn_prefill_status; // time-out code
+__device__ int g_cache_attn_prefill_range;  // 1: a length, count or page number was out of range
+
+namespace {
+
+using namespace q8;
+
+constexpr int CP_M = 128, CP_N = 128;             // query rows, keys per tile
+constexpr int CP_SOFT = 8, CP_MMA = 8, CP_CONV = 9, CP_NCONV = 3;
+constexpr int CP_THREADS = (CP_CONV + CP_NCONV) * 32;
+constexpr uint32_t CP_HALF = 128 * 128;           // [128 rows][64 FLOAT16]: 16 KB
+constexpr uint32_t CP_TMEM_COLS = 512, CP_COL_O = 256;
+constexpr float CP_TOP = 15.0f, CP_BASE = 7.0f;   // log2 of the largest p', and after a move of m
+constexpr float CP_LV_MIN = -60.0f;
+
+template <int DP> struct CpLayout {
+  static constexpr int NH = DP / 64;              // 64-column halves
+  static constexpr uint32_t TILE = NH * CP_HALF;  // a K or V operand
+  static constexpr uint32_t OFF_Q = 0;
+  static constexpr uint32_t OFF_K = TILE, OFF_V = 3 * TILE; // two buffers each
+  static constexpr uint32_t OFF_RED = 5 * TILE;             // [2][2][128] floats
+  static constexpr uint32_t OFF_SC = OFF_RED + 2 * 2 * CP_M * 4;  // float4 [4 tiles][8 chunks]
+  static constexpr uint32_t OFF_ROW = OFF_SC + 4 * 8 * 16;        // int64 [2][128]: first code of a key's row, or -1
+  static constexpr uint32_t OFF_BAR = OFF_ROW + 2 * CP_N * 8;
+  static constexpr int NBAR = 16;
+  static constexpr size_t SMEM = OFF_BAR + NBAR * 8 + 16;
+};
+
+struct CpArgs {
+  CaArgs c;
+  int qtiles, pk, np, hpacks;
+  float scale_log2;
+};
+
+// Four codes -> two FLOAT16 pairs, exactly.
+template <typename Q> __device__ __forceinline__ void widen4(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  if constexpr (std::is_same<Q, Fp8>::value) {
+    asm("{\n\t.reg .b16 a, b;\n\t"
+        "mov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  } else {
+    const uint32_t u = w ^ 0x80808080u; // 1024 + (code + 128), minus 1152
+    const __half2 k = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), k);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2 *>(&b), k);
+    lo = *reinterpret_cast<const uint32_t *>(&x);
+    hi = *reinterpret_cast<const uint32_t *>(&y);
+  }
+}
+
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+template <typename T, typename Q, int DP>
+__global__ void __launch_bounds__(CP_THREADS, 1) cache_attn_prefill(const CpArgs g) {
+  using L = CpLayout<DP>;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  if (tc::smem_u32(sm) & 1023u) { // the operands need a 1024-byte aligned base
+    if (threadIdx.x == 0) atomicExch(&g_cache_attn_prefill_status, tc::kTimeoutFull);
+    return;
+  }
+  const CaArgs &a = g.c;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sm + L::OFF_BAR);
+  float *red = reinterpret_cast<float *>(sm + L::OFF_RED);
+  float4 *sc = reinterpret_cast<float4 *>(sm + L::OFF_SC);
+  int64_t *rowoff = reinterpret_cast<int64_t *>(sm + L::OFF_ROW);
+  uint64_t *q_full = bars;       // 1
+  uint64_t *k_full = bars + 1;   // 2
+  uint64_t *k_empty = bars + 3;  // 2: S of the buffer's tile done
+  uint64_t *v_full = bars + 5;   // 2
+  uint64_t *v_empty = bars + 7;  // 2: P.V of the buffer's tile done
+  uint64_t *s_full = bars + 9;   // 2
+  uint64_t *p_full = bars + 11;  // 2
+  uint64_t *o_done = bars + 13;  // 2
+  uint64_t *mma_done = bars + 15;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::NBAR);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int qt = g.qtiles - 1 - (int)(blockIdx.x % g.qtiles); // long rows first
+  const int bhp = (int)(blockIdx.x / g.qtiles);
+  const int b = bhp / g.hpacks, h0 = (bhp % g.hpacks) * g.pk, kvh = h0 / a.group;
+  const int q0 = qt * g.np;
+  bool bad;
+  const CaSpan sp = ca_span(a, b, &bad);
+  if (bad && threadIdx.x == 0) atomicExch(&g_cache_attn_prefill_range, 1);
+  T *yb = static_cast<T *>(a.y) + (int64_t)b * a.q_b;
+  if (q0 >= sp.count) { // no query of this tile counts
+    const int cols = a.D / 8;
+    for (int e = threadIdx.x; e < CP_M * cols; e += CP_THREADS) {
+      const int row = e / cols, i = q0 + row % g.np;
+      if (i < a.S)
+        *reinterpret_cast<uint4 *>(yb + (int64_t)(h0 + row / g.np) * a.q_h + (int64_t)i * a.q_s + e % cols * 8) =
+            make_uint4(0u, 0u, 0u, 0u);
+    }
+    return;
+  }
+  // positions of the first and last query that counts; the tiles some of them see
+  const int p_first = sp.past + q0, p_last = sp.past + min(q0 + g.np, sp.count) - 1;
+  const int kend = a.causal ? min(sp.total, p_last + 1) : sp.total;
+  const bool win = a.causal && a.window >= 0;
+  const int first = win ? max(0, p_first - a.window) / CP_N : 0;
+  const int sink_tiles = win ? min((min(a.sinks, kend) + CP_N - 1) / CP_N, first) : 0;
+  const int ntiles = sink_tiles + (kend + CP_N - 1) / CP_N - first;
+  auto key0_of = [&](int j) { return (j < sink_tiles ? j : first + j - sink_tiles) * CP_N; };
+
+  if (threadIdx.x == 0) {
+    tc::mbar_init(q_full, CP_SOFT);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&k_full[i], CP_NCONV);
+      tc::mbar_init(&k_empty[i], 1);
+      tc::mbar_init(&v_full[i], CP_NCONV);
+      tc::mbar_init(&v_empty[i], 1);
+      tc::mbar_init(&s_full[i], 1);
+      tc::mbar_init(&p_full[i], CP_SOFT);
+      tc::mbar_init(&o_done[i], 1);
+    }
+    tc::mbar_init(mma_done, 1);
+    *abort_flag = 0;
+    tc::fence_barrier_init();
+  }
+  if (warp == CP_MMA) {
+    tc::tmem_alloc(tmem_slot, CP_TMEM_COLS);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= CP_CONV) {
+    // ------------------------------ converters --------------------------------
+    // Threads 0..95 look after keys ct, ct + 96 of each tile: the place of the key's codes goes to
+    // rowoff, two tiles deep, and every 16th key's page scales to sc, four deep (the softmax of a
+    // tile reads them while the converters are up to three tiles ahead).
+    const int ct = threadIdx.x - CP_CONV * 32, cw = warp - CP_CONV;
+    constexpr int CT = CP_NCONV * 32;
+    auto conv_sync = [] { asm volatile("bar.sync 2, %0;" ::"n"(CP_NCONV * 32) : "memory"); };
+    auto page_of = [&](int j, int r) -> int { // page of key r of tile j; -1: the sequence has no such key
+      if (j >= ntiles || r >= CP_N) return -1;
+      const int key = key0_of(j) + r;
+      return key < sp.total ? a.table[(int64_t)b * a.max_pages + key / a.T] : -1;
+    };
+    auto note = [&](int j, int r, int id) {
+      if (j >= ntiles || r >= CP_N) return;
+      const int key = key0_of(j) + r;
+      const bool has = key < sp.total, ok = has && id >= 0 && id < a.pages;
+      if (has && !ok) atomicExch(&g_cache_attn_prefill_range, 1);
+      const int64_t z = (int64_t)id * a.Hkv + kvh;
+      rowoff[(j & 1) * CP_N + r] = ok ? (z * a.T + key % a.T) * a.D : -1;
+      if (r % 16 == 0) {
+        float4 c = make_float4(0.0f, CP_LV_MIN, 0.0f, 0.0f);
+        if (ok) {
+          const float ks = a.ks[z] * g.scale_log2, vs = a.vs[z];
+          c.x = ks;
+          c.y = fmaxf(log2f(vs), CP_LV_MIN); // a NaN gives the bound
+          c.z = exp2f(-c.y);
+          // 1: scales of ordinary values; 2: the softmax looks at each score
+          const bool plain = ks > 0.0f && ks < INFINITY && fabsf(vs) < INFINITY;
+          c.w = plain ? 1.0f : 2.0f;
+          if (!(fabsf(vs) < INFINITY)) c.z = __uint_as_float(0x7fc00000u);
+        }
+        sc[(j & 3) * 8 + r / 16] = c;
+      }
+    };
+    // 16-code units: lanes cover DP / 16 units of 512 / DP keys; a warp takes every third group
+    constexpr int UPR = DP / 16, KPW = 32 / UPR, GROUPS = CP_N / KPW, MINE = (GROUPS + CP_NCONV - 1) / CP_NCONV;
+    const int u = lane % UPR, sub = lane / UPR;
+    const bool has_cols = u * 16 < a.D;
+    uint4 kr[MINE], vr[MINE];
+    auto load = [&](const uint8_t *pool, int j, uint4 (&r)[MINE]) {
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        const int grp = cw + i * CP_NCONV;
+        r[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (grp < GROUPS && has_cols) {
+          const int64_t off = rowoff[(j & 1) * CP_N + grp * KPW + sub];
+          if (off >= 0) r[i] = __ldg(reinterpret_cast<const uint4 *>(pool + off + u * 16));
+        }
+      }
+    };
+    // zero codes widen to zeros, so keys without a token and columns past D become zeros
+    auto store = [&](uint32_t base, int j, const uint4 (&r)[MINE], bool values) {
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        const int grp = cw + i * CP_NCONV, row = grp * KPW + sub;
+        if (grp < GROUPS) {
+          const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+          uint32_t h[8];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) widen4<Q>(w[q], h[2 * q], h[2 * q + 1]);
+          if (values) {
+            const float lv = sc[(j & 3) * 8 + row / 16].y;
+            if (lv <= CP_LV_MIN) { // a value scale below 2^-60: what 2^lv does not hold goes into the codes
+              const int64_t off = rowoff[(j & 1) * CP_N + row];
+              const float vs = off >= 0 ? a.vs[off / a.D / a.T] : 0.0f;
+              const float f = fabsf(vs) < INFINITY ? vs * exp2f(-CP_LV_MIN) : 0.0f;
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&h[q]));
+                h[q] = half2_of(v.x * f, v.y * f);
+              }
+            }
+          }
+          uint8_t *p = sm + base + (u >> 2) * CP_HALF + row * 128;
+          const int c = (u & 3) * 2;
+          *reinterpret_cast<uint4 *>(p + ((c ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4 *>(p + (((c + 1) ^ (row & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+      }
+    };
+    int id0 = page_of(0, ct), id1 = page_of(0, ct + CT);
+    note(0, ct, id0);
+    note(0, ct + CT, id1);
+    id0 = page_of(1, ct);
+    id1 = page_of(1, ct + CT);
+    conv_sync();
+    load(a.k, 0, kr);
+    bool ok = true;
+    for (int j = 0; j < ntiles; ++j) {
+      const int s = j & 1;
+      load(a.v, j, vr);
+      // the next tile's places (the buffer's last reader was this warp group's V of tile j - 1)
+      note(j + 1, ct, id0);
+      note(j + 1, ct + CT, id1);
+      id0 = page_of(j + 2, ct);
+      id1 = page_of(j + 2, ct + CT);
+      if (ok && (*abort_flag || (j >= 2 && !tc::mbar_wait(&k_empty[s], ((j - 2) >> 1) & 1)))) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        store(L::OFF_K + s * L::TILE, j, kr, false);
+        tc::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&k_full[s]);
+      }
+      conv_sync(); // rowoff and sc of tile j + 1 are written
+      if (j + 1 < ntiles) load(a.k, j + 1, kr);
+      if (ok && (*abort_flag || (j >= 2 && !tc::mbar_wait(&v_empty[s], ((j - 2) >> 1) & 1)))) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        store(L::OFF_V + s * L::TILE, j, vr, true);
+        tc::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&v_full[s]);
+      }
+      conv_sync(); // every warp is done with rowoff of tile j
+    }
+    if (!ok && lane == 0 && !*abort_flag) {
+      atomicExch(&g_cache_attn_prefill_status, tc::kTimeoutEmpty);
+      *abort_flag = 1;
+    }
+  } else if (warp == CP_MMA) {
+    // ------------------------------ MMA issuer --------------------------------
+    if (tc::elect_one()) {
+      const uint32_t id_s = tc::idesc(1, 0, 0, 0, 0, CP_M, CP_N);
+      const uint32_t id_o = tc::idesc(1, 0, 0, 0, 1, CP_M, DP);
+      const uint32_t q_base = tc::smem_u32(sm + L::OFF_Q);
+      bool ok = tc::mbar_wait(q_full, 0);
+      auto issue_pv = [&](int j) { // O (+)= P_j V_j, V read MN-major over the head's columns
+        if (!tc::mbar_wait(&p_full[j & 1], (j >> 1) & 1)) return false;
+        if (!tc::mbar_wait(&v_full[j & 1], (j >> 1) & 1)) return false;
+        tc::tc_fence_after();
+        const uint32_t p_col = tmem + (uint32_t)(j & 1) * CP_N;
+        const uint32_t v_base = tc::smem_u32(sm + L::OFF_V + (j & 1) * L::TILE);
+#pragma unroll
+        for (int kk = 0; kk < CP_N / 16; ++kk) {
+          const uint64_t bd = tc::sdesc_sw128(v_base + kk * 16 * 128, CP_HALF, 1024);
+          tc::mma_f16_ts(tmem + CP_COL_O, p_col + kk * 8, bd, id_o, (j > 0 || kk > 0) ? 1u : 0u);
+        }
+        tc::tc_commit(&o_done[j & 1]);
+        tc::tc_commit(&v_empty[j & 1]);
+        return true;
+      };
+      for (int j = 0; ok && j < ntiles; ++j) {
+        if (*abort_flag || !tc::mbar_wait(&k_full[j & 1], (j >> 1) & 1)) {
+          ok = false;
+          break;
+        }
+        // S buffer j & 1 holds P_{j-2} until P.V of tile j - 2 is done
+        if (j >= 2 && !tc::mbar_wait(&o_done[j & 1], ((j - 2) >> 1) & 1)) {
+          ok = false;
+          break;
+        }
+        tc::tc_fence_after();
+        const uint32_t k_base = tc::smem_u32(sm + L::OFF_K + (j & 1) * L::TILE);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint64_t ad = tc::sdesc_sw128(q_base + (kk >> 2) * CP_HALF + (kk & 3) * 32, 16, 1024);
+          const uint64_t bd = tc::sdesc_sw128(k_base + (kk >> 2) * CP_HALF + (kk & 3) * 32, 16, 1024);
+          tc::mma_f16(tmem + (j & 1) * CP_N, ad, bd, id_s, kk > 0 ? 1u : 0u);
+        }
+        tc::tc_commit(&s_full[j & 1]);
+        tc::tc_commit(&k_empty[j & 1]);
+        if (j >= 1 && !issue_pv(j - 1)) ok = false;
+      }
+      if (ok && !issue_pv(ntiles - 1)) ok = false;
+      if (!ok) {
+        atomicExch(&g_cache_attn_prefill_status, tc::kTimeoutFull);
+        *abort_flag = 1;
+      }
+      // TMEM is freed below: wait (bounded) until every issued MMA is done
+      tc::tc_commit(mma_done);
+      tc::mbar_wait(mma_done, 0);
+    }
+  } else {
+    // ------------------------------ softmax warps -----------------------------
+    // Warps w and w + 4 share TMEM lanes 32 (w % 4) .. + 31; each thread has one half of its row's
+    // columns.  Control flow stays warp-uniform around the TMEM accesses, and every softmax warp
+    // takes every named barrier even after a time-out, so none can hang.
+    const int quarter = warp & 3, half = warp >> 2;
+    const int row = quarter * 32 + lane;           // query row = TMEM lane
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const int qi = q0 + row % g.np, pos = sp.past + qi; // position of the row's query
+    const bool counts = qi < sp.count;
+    auto softmax_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(CP_SOFT * 32) : "memory"); };
+    float qf = 1.0f; // power of two taken out of the row's queries
+    {
+      // this thread's 64 columns of Q -> FLOAT16 in the swizzled operand
+      uint32_t w[32];
+      const T *qp = static_cast<const T *>(a.q) + (int64_t)b * a.q_b + (int64_t)(h0 + row / g.np) * a.q_h +
+                    (int64_t)qi * a.q_s;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const int d = half * 64 + c * 8;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (counts && d < a.D) v = __ldg(reinterpret_cast<const uint4 *>(qp + d));
+        w[4 * c] = v.x;
+        w[4 * c + 1] = v.y;
+        w[4 * c + 2] = v.z;
+        w[4 * c + 3] = v.w;
+      }
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        uint32_t e = 0u;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) e = max(e, max(w[c] & 0x7f80u, (w[c] >> 16) & 0x7f80u));
+        uint32_t *re = reinterpret_cast<uint32_t *>(red);
+        re[half * CP_M + row] = e;
+        softmax_sync();
+        e = max(e, re[(half ^ 1) * CP_M + row]);
+        softmax_sync(); // red is free again
+        const int ex = min(max((int)(e >> 7) - 127, -126), 126);
+        const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
+        qf = __uint_as_float((uint32_t)(127 + ex) << 23);
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+          w[c] = half2_of(__uint_as_float(w[c] << 16) * down, __uint_as_float(w[c] & 0xffff0000u) * down);
+      }
+      if (half < L::NH) {
+        uint8_t *p = sm + L::OFF_Q + half * CP_HALF + row * 128;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4 *>(p + ((c ^ (row & 7)) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+      }
+      tc::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(q_full);
+    }
+    float m_ref = -INFINITY, l_part = 0.0f;
+    bool ok = true;
+    auto uniform_wait = [&](uint64_t *bar, uint32_t parity) {
+      const bool w = ok && !*abort_flag && tc::mbar_wait(bar, parity);
+      return __all_sync(0xffffffffu, w);
+    };
+    constexpr int OC = DP / 2; // O columns per thread
+    for (int j = 0; j < ntiles; ++j) {
+      if (!uniform_wait(&s_full[j & 1], (j >> 1) & 1)) ok = false;
+      tc::tc_fence_after();
+      const int key0 = key0_of(j) + half * 64;
+      const uint32_t s_col = tmem + lane_off + (j & 1) * CP_N + half * 64;
+      // the scores of this half row stay in registers; vk, lv: factor and offset of each 16 keys' exponents
+      float v[64], vk[4], lv[4], inv[4];
+      float mx = -INFINITY;
+      bool poison = false;
+      if (ok) {
+        bool plain = g.scale_log2 > 0.0f && a.softcap <= 0.0f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float4 f = sc[(j & 3) * 8 + half * 4 + c];
+          vk[c] = f.x * qf;
+          lv[c] = f.y;
+          inv[c] = f.z;
+          plain = plain && f.w == 1.0f;
+        }
+        const bool need_mask = key0 + 64 > sp.total || (a.causal && key0 + 63 > p_first) ||
+                               (win && key0 < p_last - a.window && key0 + 64 > a.sinks);
+        uint32_t r0[32], r1[32];
+        tc::tmem_ld32(s_col, r0);
+        tc::tmem_ld32(s_col + 32, r1);
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          v[e] = __uint_as_float(r0[e]);
+          v[32 + e] = __uint_as_float(r1[e]);
+        }
+        if (!__all_sync(0xffffffffu, plain && !need_mask)) {
+          // every score in base-2 units, -inf where the row does not see the key; pages out of
+          // range (flag 0) hold no keys
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float flag = sc[(j & 3) * 8 + half * 4 + c].w;
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int key = key0 + c * 16 + e;
+              float x = v[c * 16 + e] * vk[c];
+              if (a.softcap > 0.0f) x = a.softcap * tanhf(x * kLn2 / a.softcap) * kLog2E;
+              const bool seen = flag != 0.0f && key < sp.total && ca_sees(a, pos, key);
+              any = any || seen;
+              v[c * 16 + e] = seen ? x : -INFINITY;
+            }
+            poison = poison || (any && inv[c] != inv[c]); // it sees values that are not finite
+            if (inv[c] != inv[c]) inv[c] = 0.0f;
+            vk[c] = 1.0f;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float m = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) m = max3f(m, v[c * 16 + e], v[c * 16 + e + 1]);
+          mx = fmaxf(mx, fmaf(m, vk[c], lv[c])); // vk > 0
+        }
+      }
+      float *rm = red + (j & 1) * 2 * CP_M;
+      rm[half * CP_M + row] = mx;
+      softmax_sync();
+      mx = fmaxf(mx, rm[(half ^ 1) * CP_M + row]);
+      if (!ok) continue;
+      const bool reb = mx > m_ref + CP_TOP;
+      float corr = 1.0f;
+      if (reb) {
+        const float to = mx - CP_BASE;
+        corr = exp2f(m_ref - to);
+        l_part *= corr;
+        m_ref = to;
+      }
+      if (j >= 1 && __any_sync(0xffffffffu, reb)) {
+        if (!uniform_wait(&o_done[(j - 1) & 1], ((j - 1) >> 1) & 1)) {
+          ok = false;
+          continue;
+        }
+        tc::tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < OC / 32; ++c) {
+          const uint32_t o_col = tmem + lane_off + CP_COL_O + half * OC + c * 32;
+          uint32_t r[32];
+          tc::tmem_ld32(o_col, r);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * corr);
+          tc::tmem_st32(o_col, r);
+        }
+        tc::tmem_st_wait();
+      }
+      // P over the S buffer the scores came from (every thread of the row has read its S half
+      // before the barrier above)
+      const float ref = m_ref == -INFINITY ? 0.0f : m_ref;
+      const uint32_t p_col = tmem + lane_off + (j & 1) * CP_N + half * 32;
+#pragma unroll
+      for (int c2 = 0; c2 < 2; ++c2) {
+        uint32_t ph[16];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int c = c2 * 2 + h;
+          const uint64_t k2 = f2pack(vk[c], vk[c]), o2 = f2pack(lv[c] - ref, lv[c] - ref);
+          uint64_t ls = f2pack(0.0f, 0.0f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float2 x = f2unpack(ffma2(f2pack(v[c * 16 + 2 * e], v[c * 16 + 2 * e + 1]), k2, o2));
+            const float p0 = ex2(x.x), p1 = ex2(x.y);
+            ls = fadd2(ls, f2pack(p0, p1));
+            ph[h * 8 + e] = half2_of(p0, p1);
+          }
+          const float2 l2 = f2unpack(ls);
+          l_part = fmaf(l2.x + l2.y, inv[c], l_part);
+        }
+        tc::tmem_st16(p_col + c2 * 16, ph);
+      }
+      if (poison) l_part = __uint_as_float(0x7fc00000u);
+      tc::tmem_st_wait();
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&p_full[j & 1]);
+    }
+    const int last = ntiles - 1;
+    const bool fin = uniform_wait(&o_done[last & 1], (last >> 1) & 1);
+    softmax_sync();
+    red[half * CP_M + row] = l_part;
+    softmax_sync();
+    const float l_sum = l_part + red[(half ^ 1) * CP_M + row];
+    if (fin) {
+      tc::tc_fence_after();
+      const float scale = l_sum == 0.0f ? 0.0f : 1.0f / l_sum; // a NaN stays
+      T *yr = yb + (int64_t)(h0 + row / g.np) * a.q_h + (int64_t)qi * a.q_s;
+      uint32_t r[32];
+#pragma unroll 1
+      for (int c = 0; c < OC / 32; ++c) {
+        tc::tmem_ld32(tmem + lane_off + CP_COL_O + half * OC + c * 32, r);
+        tc::tmem_ld_wait();
+        if (qi < a.S) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int d = half * OC + c * 32 + q * 8;
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = counts ? __uint_as_float(r[q * 8 + e]) * scale : 0.0f;
+            if (d < a.D) Raw8<T>::store(yr + d, f);
+          }
+        }
+      }
+    } else {
+      atomicExch(&g_cache_attn_prefill_status, tc::kTimeoutFull);
+      *abort_flag = 1;
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == CP_MMA) tc::tmem_dealloc(tmem, CP_TMEM_COLS);
+}
+
+int cp_pk(int group) { // heads per CTA
+  int pk = 1;
+  while (pk < 8 && group % (2 * pk) == 0) pk *= 2;
+  return pk;
+}
+
+template <typename T, typename Q> int cp_launch(const CpArgs &g, unsigned grid, cudaStream_t st) {
+  if (g.c.D <= 64) {
+    auto kern = cache_attn_prefill<T, Q, 64>;
+    B2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)CpLayout<64>::SMEM));
+    kern<<<grid, CP_THREADS, CpLayout<64>::SMEM, st>>>(g);
+  } else {
+    auto kern = cache_attn_prefill<T, Q, 128>;
+    B2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)CpLayout<128>::SMEM));
+    kern<<<grid, CP_THREADS, CpLayout<128>::SMEM, st>>>(g);
+  }
+  B2_LAUNCH_CHECK();
+  return B2_OK;
+}
+
+int cp_read(int reset, const int &symbol) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, symbol, sizeof(int)) != cudaSuccess) return -1;
+  if (reset && v) {
+    const int z = 0;
+    if (cudaMemcpyToSymbol(symbol, &z, sizeof(int)) != cudaSuccess) return -1;
+  }
+  return v;
+}
+
+} // namespace
+
+// CTAs of a call.
+int64_t cache_attn_prefill_ctas(const CaArgs &a) {
+  const int pk = cp_pk(a.group), np = CP_M / pk;
+  return (int64_t)((a.S + np - 1) / np) * a.B * (a.Hq / pk);
+}
+
+bool cache_attn_prefill_eligible(const CaArgs &a) {
+  return a.D % 16 == 0 && a.D <= 128 && a.T % 16 == 0 && aligned(a.q, 16) && aligned(a.y, 16) && aligned(a.k, 16) &&
+         aligned(a.v, 16) && a.q_h % 8 == 0 && a.q_s % 8 == 0 && cache_attn_prefill_ctas(a) < ((int64_t)1 << 31);
+}
+
+int cache_attn_prefill_launch(const CaArgs &a, bool f16, bool f8, cudaStream_t st) {
+  CpArgs g{};
+  g.c = a;
+  g.pk = cp_pk(a.group);
+  g.np = CP_M / g.pk;
+  g.qtiles = (a.S + g.np - 1) / g.np;
+  g.hpacks = a.Hq / g.pk;
+  g.scale_log2 = a.scale * kLog2E;
+  const unsigned grid = (unsigned)cache_attn_prefill_ctas(a);
+  if (f16) return f8 ? cp_launch<__half, Fp8>(g, grid, st) : cp_launch<__half, Int8>(g, grid, st);
+  return f8 ? cp_launch<__nv_bfloat16, Fp8>(g, grid, st) : cp_launch<__nv_bfloat16, Int8>(g, grid, st);
+}
+
+int status_read_cache_attn_prefill(int reset) { return cp_read(reset, g_cache_attn_prefill_status); }
+int range_read_cache_attn_prefill(int reset) { return cp_read(reset, g_cache_attn_prefill_range); }
+
+} // namespace b2

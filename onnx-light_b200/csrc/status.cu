@@ -34,6 +34,8 @@ int status_read_cache_attention(int reset);
 int status_read_scaled_tc(int reset);
 int status_read_cache_attn_split(int reset);
 int range_read_cache_attn_split(int reset);
+int status_read_cache_attn_prefill(int reset);
+int range_read_cache_attn_prefill(int reset);
 
 __device__ int g_selftest_status;
 
@@ -78,7 +80,9 @@ extern "C" B2_API int b2_kernel_status(int reset) {
                       {"b200::KVCacheAppend", status_read_cache_append, kCacheRange},
                       {"b200::QuantizedCacheAttention", status_read_cache_attention, kCacheRange},
                       {"b200::QuantizedCacheAttention", range_read_cache_attn_split, kCacheRange},
+                      {"b200::QuantizedCacheAttention", range_read_cache_attn_prefill, kCacheRange},
                       {"cache_attn_split", status_read_cache_attn_split, 0},
+                      {"cache_attn_prefill", status_read_cache_attn_prefill, 0},
                       {"scaled_mm_tc", status_read_scaled_tc, 0}};
   int first = 0;
   for (const Src &s : srcs) {
