@@ -6,7 +6,7 @@
 // One CTA owns 128 query rows -- pk heads of one GQA group (pk the largest power of two up to 8 that
 // divides the group) x 128 / pk positions -- and walks the 128-key tiles that any of them sees (the
 // sinks' tiles, then the window's up to the diagonal):
-//   warps 9-11 (converters) read the tile's codes from their pages, 16 bytes a lane, widen them to
+//   warps 9-15 (converters) read the tile's codes from their pages, 16 bytes a lane, widen them to
 //              FLOAT16 (exact for both code types) and write the 128-byte-swizzled K and V
 //              operands, two buffers each; rows that hold no token become zeros;
 //   warp 8     (MMA) issues S = Q K^T into one of two TMEM buffers and O += P V with P read from TMEM;
@@ -37,7 +37,10 @@ namespace {
 using namespace q8;
 
 constexpr int CP_M = 128, CP_N = 128;             // query rows, keys per tile
-constexpr int CP_SOFT = 8, CP_MMA = 8, CP_CONV = 9, CP_NCONV = 3;
+constexpr int CP_SOFT = 8, CP_MMA = 8, CP_CONV = 9, CP_NCONV = 7;
+// Registers: 16 warps start with 128 each; the two softmax warpgroups take 168, the other two keep
+// 88 (2 x 168 + 2 x 88 = 4 x 128).
+constexpr int CP_REG_SOFT = 168, CP_REG_REST = 88;
 constexpr int CP_THREADS = (CP_CONV + CP_NCONV) * 32;
 constexpr uint32_t CP_HALF = 128 * 128;           // [128 rows][64 FLOAT16]: 16 KB
 constexpr uint32_t CP_TMEM_COLS = 512, CP_COL_O = 256;
@@ -61,6 +64,7 @@ struct CpArgs {
   CaArgs c;
   int qtiles, pk, np, hpacks;
   float scale_log2;
+  FastDiv div_t; // by the page size
 };
 
 // Four codes -> two FLOAT16 pairs, exactly.
@@ -165,181 +169,179 @@ __global__ void __launch_bounds__(CP_THREADS, 1) cache_attn_prefill(const CpArgs
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= CP_CONV) {
-    // ------------------------------ converters --------------------------------
-    // Threads 0..95 look after keys ct, ct + 96 of each tile: the place of the key's codes goes to
-    // rowoff, two tiles deep, and every 16th key's page scales to sc, four deep (the softmax of a
-    // tile reads them while the converters are up to three tiles ahead).
-    const int ct = threadIdx.x - CP_CONV * 32, cw = warp - CP_CONV;
-    constexpr int CT = CP_NCONV * 32;
-    auto conv_sync = [] { asm volatile("bar.sync 2, %0;" ::"n"(CP_NCONV * 32) : "memory"); };
-    auto page_of = [&](int j, int r) -> int { // page of key r of tile j; -1: the sequence has no such key
-      if (j >= ntiles || r >= CP_N) return -1;
-      const int key = key0_of(j) + r;
-      return key < sp.total ? a.table[(int64_t)b * a.max_pages + key / a.T] : -1;
-    };
-    auto note = [&](int j, int r, int id) {
-      if (j >= ntiles || r >= CP_N) return;
-      const int key = key0_of(j) + r;
-      const bool has = key < sp.total, ok = has && id >= 0 && id < a.pages;
-      if (has && !ok) atomicExch(&g_cache_attn_prefill_range, 1);
-      const int64_t z = (int64_t)id * a.Hkv + kvh;
-      rowoff[(j & 1) * CP_N + r] = ok ? (z * a.T + key % a.T) * a.D : -1;
-      if (r % 16 == 0) {
-        float4 c = make_float4(0.0f, CP_LV_MIN, 0.0f, 0.0f);
-        if (ok) {
-          const float ks = a.ks[z] * g.scale_log2, vs = a.vs[z];
-          c.x = ks;
-          c.y = fmaxf(log2f(vs), CP_LV_MIN); // a NaN gives the bound
-          c.z = exp2f(-c.y);
-          // 1: scales of ordinary values; 2: the softmax looks at each score
-          const bool plain = ks > 0.0f && ks < INFINITY && fabsf(vs) < INFINITY;
-          c.w = plain ? 1.0f : 2.0f;
-          if (!(fabsf(vs) < INFINITY)) c.z = __uint_as_float(0x7fc00000u);
+  if (warp >= CP_SOFT) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CP_REG_REST));
+    if (warp >= CP_CONV) {
+      // ------------------------------ converters --------------------------------
+      // The first 128 threads look after one key of each tile: the place of its codes goes to rowoff,
+      // two tiles deep, and every 16th key's page scales to sc, four deep (the softmax of a tile reads
+      // them while the converters are up to three tiles ahead).
+      const int ct = threadIdx.x - CP_CONV * 32, cw = warp - CP_CONV;
+      auto conv_sync = [] { asm volatile("bar.sync 2, %0;" ::"n"(CP_NCONV * 32) : "memory"); };
+      auto page_of = [&](int j, int r) -> int { // page of key r of tile j; -1: the sequence has no such key
+        if (j >= ntiles || r >= CP_N) return -1;
+        const int key = key0_of(j) + r;
+        return key < sp.total ? a.table[(int64_t)b * a.max_pages + g.div_t.div(key)] : -1;
+      };
+      auto note = [&](int j, int r, int id) {
+        if (j >= ntiles || r >= CP_N) return;
+        const int key = key0_of(j) + r;
+        const bool has = key < sp.total, ok = has && id >= 0 && id < a.pages;
+        if (has && !ok) atomicExch(&g_cache_attn_prefill_range, 1);
+        const int64_t z = (int64_t)id * a.Hkv + kvh;
+        rowoff[(j & 1) * CP_N + r] = ok ? (z * a.T + (key - (int)g.div_t.div(key) * a.T)) * a.D : -1;
+        if (r % 16 == 0) {
+          float4 c = make_float4(0.0f, CP_LV_MIN, 0.0f, 0.0f);
+          if (ok) {
+            const float ks = a.ks[z] * g.scale_log2, vs = a.vs[z];
+            c.x = ks;
+            c.y = fmaxf(log2f(vs), CP_LV_MIN); // a NaN gives the bound
+            c.z = exp2f(-c.y);
+            // 1: scales of ordinary values; 2: the softmax looks at each score
+            const bool plain = ks > 0.0f && ks < INFINITY && fabsf(vs) < INFINITY;
+            c.w = plain ? 1.0f : 2.0f;
+            if (!(fabsf(vs) < INFINITY)) c.z = __uint_as_float(0x7fc00000u);
+          }
+          sc[(j & 3) * 8 + r / 16] = c;
         }
-        sc[(j & 3) * 8 + r / 16] = c;
-      }
-    };
-    // 16-code units: lanes cover DP / 16 units of 512 / DP keys; a warp takes every third group
-    constexpr int UPR = DP / 16, KPW = 32 / UPR, GROUPS = CP_N / KPW, MINE = (GROUPS + CP_NCONV - 1) / CP_NCONV;
-    const int u = lane % UPR, sub = lane / UPR;
-    const bool has_cols = u * 16 < a.D;
-    uint4 kr[MINE], vr[MINE];
-    auto load = [&](const uint8_t *pool, int j, uint4 (&r)[MINE]) {
-#pragma unroll
-      for (int i = 0; i < MINE; ++i) {
-        const int grp = cw + i * CP_NCONV;
-        r[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (grp < GROUPS && has_cols) {
-          const int64_t off = rowoff[(j & 1) * CP_N + grp * KPW + sub];
-          if (off >= 0) r[i] = __ldg(reinterpret_cast<const uint4 *>(pool + off + u * 16));
+      };
+      // 16-code units: lanes cover DP / 16 units of 512 / DP keys; a warp takes every seventh group
+      constexpr int UPR = DP / 16, KPW = 32 / UPR, GROUPS = CP_N / KPW, MINE = (GROUPS + CP_NCONV - 1) / CP_NCONV;
+      const int u = lane % UPR, sub = lane / UPR;
+      const bool has_cols = u * 16 < a.D;
+      uint4 kr[MINE], vr[MINE];
+      auto load = [&](const uint8_t *pool, int j, uint4 (&r)[MINE]) {
+  #pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+          const int grp = cw + i * CP_NCONV;
+          r[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (grp < GROUPS && has_cols) {
+            const int64_t off = rowoff[(j & 1) * CP_N + grp * KPW + sub];
+            if (off >= 0) r[i] = __ldg(reinterpret_cast<const uint4 *>(pool + off + u * 16));
+          }
         }
-      }
-    };
-    // zero codes widen to zeros, so keys without a token and columns past D become zeros
-    auto store = [&](uint32_t base, int j, const uint4 (&r)[MINE], bool values) {
-#pragma unroll
-      for (int i = 0; i < MINE; ++i) {
-        const int grp = cw + i * CP_NCONV, row = grp * KPW + sub;
-        if (grp < GROUPS) {
-          const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
-          uint32_t h[8];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) widen4<Q>(w[q], h[2 * q], h[2 * q + 1]);
-          if (values) {
-            const float lv = sc[(j & 3) * 8 + row / 16].y;
-            if (lv <= CP_LV_MIN) { // a value scale below 2^-60: what 2^lv does not hold goes into the codes
-              const int64_t off = rowoff[(j & 1) * CP_N + row];
-              const float vs = off >= 0 ? a.vs[off / a.D / a.T] : 0.0f;
-              const float f = fabsf(vs) < INFINITY ? vs * exp2f(-CP_LV_MIN) : 0.0f;
-#pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&h[q]));
-                h[q] = half2_of(v.x * f, v.y * f);
+      };
+      // zero codes widen to zeros, so keys without a token and columns past D become zeros
+      auto store = [&](uint32_t base, int j, const uint4 (&r)[MINE], bool values) {
+  #pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+          const int grp = cw + i * CP_NCONV, row = grp * KPW + sub;
+          if (grp < GROUPS) {
+            const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+            uint32_t h[8];
+  #pragma unroll
+            for (int q = 0; q < 4; ++q) widen4<Q>(w[q], h[2 * q], h[2 * q + 1]);
+            if (values) {
+              const float lv = sc[(j & 3) * 8 + row / 16].y;
+              if (lv <= CP_LV_MIN) { // a value scale below 2^-60: what 2^lv does not hold goes into the codes
+                const int64_t off = rowoff[(j & 1) * CP_N + row];
+                const float vs = off >= 0 ? a.vs[off / a.D / a.T] : 0.0f;
+                const float f = fabsf(vs) < INFINITY ? vs * exp2f(-CP_LV_MIN) : 0.0f;
+  #pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                  const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&h[q]));
+                  h[q] = half2_of(v.x * f, v.y * f);
+                }
               }
             }
+            uint8_t *p = sm + base + (u >> 2) * CP_HALF + row * 128;
+            const int c = (u & 3) * 2;
+            *reinterpret_cast<uint4 *>(p + ((c ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4 *>(p + (((c + 1) ^ (row & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
           }
-          uint8_t *p = sm + base + (u >> 2) * CP_HALF + row * 128;
-          const int c = (u & 3) * 2;
-          *reinterpret_cast<uint4 *>(p + ((c ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-          *reinterpret_cast<uint4 *>(p + (((c + 1) ^ (row & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
         }
-      }
-    };
-    int id0 = page_of(0, ct), id1 = page_of(0, ct + CT);
-    note(0, ct, id0);
-    note(0, ct + CT, id1);
-    id0 = page_of(1, ct);
-    id1 = page_of(1, ct + CT);
-    conv_sync();
-    load(a.k, 0, kr);
-    bool ok = true;
-    for (int j = 0; j < ntiles; ++j) {
-      const int s = j & 1;
-      load(a.v, j, vr);
-      // the next tile's places (the buffer's last reader was this warp group's V of tile j - 1)
-      note(j + 1, ct, id0);
-      note(j + 1, ct + CT, id1);
-      id0 = page_of(j + 2, ct);
-      id1 = page_of(j + 2, ct + CT);
-      if (ok && (*abort_flag || (j >= 2 && !tc::mbar_wait(&k_empty[s], ((j - 2) >> 1) & 1)))) ok = false;
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
-        store(L::OFF_K + s * L::TILE, j, kr, false);
-        tc::fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&k_full[s]);
-      }
-      conv_sync(); // rowoff and sc of tile j + 1 are written
-      if (j + 1 < ntiles) load(a.k, j + 1, kr);
-      if (ok && (*abort_flag || (j >= 2 && !tc::mbar_wait(&v_empty[s], ((j - 2) >> 1) & 1)))) ok = false;
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
-        store(L::OFF_V + s * L::TILE, j, vr, true);
-        tc::fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&v_full[s]);
-      }
-      conv_sync(); // every warp is done with rowoff of tile j
-    }
-    if (!ok && lane == 0 && !*abort_flag) {
-      atomicExch(&g_cache_attn_prefill_status, tc::kTimeoutEmpty);
-      *abort_flag = 1;
-    }
-  } else if (warp == CP_MMA) {
-    // ------------------------------ MMA issuer --------------------------------
-    if (tc::elect_one()) {
-      const uint32_t id_s = tc::idesc(1, 0, 0, 0, 0, CP_M, CP_N);
-      const uint32_t id_o = tc::idesc(1, 0, 0, 0, 1, CP_M, DP);
-      const uint32_t q_base = tc::smem_u32(sm + L::OFF_Q);
-      bool ok = tc::mbar_wait(q_full, 0);
-      auto issue_pv = [&](int j) { // O (+)= P_j V_j, V read MN-major over the head's columns
-        if (!tc::mbar_wait(&p_full[j & 1], (j >> 1) & 1)) return false;
-        if (!tc::mbar_wait(&v_full[j & 1], (j >> 1) & 1)) return false;
-        tc::tc_fence_after();
-        const uint32_t p_col = tmem + (uint32_t)(j & 1) * CP_N;
-        const uint32_t v_base = tc::smem_u32(sm + L::OFF_V + (j & 1) * L::TILE);
-#pragma unroll
-        for (int kk = 0; kk < CP_N / 16; ++kk) {
-          const uint64_t bd = tc::sdesc_sw128(v_base + kk * 16 * 128, CP_HALF, 1024);
-          tc::mma_f16_ts(tmem + CP_COL_O, p_col + kk * 8, bd, id_o, (j > 0 || kk > 0) ? 1u : 0u);
-        }
-        tc::tc_commit(&o_done[j & 1]);
-        tc::tc_commit(&v_empty[j & 1]);
-        return true;
       };
-      for (int j = 0; ok && j < ntiles; ++j) {
-        if (*abort_flag || !tc::mbar_wait(&k_full[j & 1], (j >> 1) & 1)) {
-          ok = false;
-          break;
+      note(0, ct, page_of(0, ct));
+      int id = page_of(1, ct);
+      conv_sync();
+      load(a.k, 0, kr);
+      bool ok = true;
+      for (int j = 0; j < ntiles; ++j) {
+        const int s = j & 1;
+        load(a.v, j, vr);
+        // the next tile's places (the buffer's last reader was this warp group's V of tile j - 1)
+        note(j + 1, ct, id);
+        id = page_of(j + 2, ct);
+        if (ok && (*abort_flag || (j >= 2 && !tc::mbar_wait(&k_empty[s], ((j - 2) >> 1) & 1)))) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+          store(L::OFF_K + s * L::TILE, j, kr, false);
+          tc::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&k_full[s]);
         }
-        // S buffer j & 1 holds P_{j-2} until P.V of tile j - 2 is done
-        if (j >= 2 && !tc::mbar_wait(&o_done[j & 1], ((j - 2) >> 1) & 1)) {
-          ok = false;
-          break;
+        conv_sync(); // rowoff and sc of tile j + 1 are written
+        if (j + 1 < ntiles) load(a.k, j + 1, kr);
+        if (ok && (*abort_flag || (j >= 2 && !tc::mbar_wait(&v_empty[s], ((j - 2) >> 1) & 1)))) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+          store(L::OFF_V + s * L::TILE, j, vr, true);
+          tc::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&v_full[s]);
         }
-        tc::tc_fence_after();
-        const uint32_t k_base = tc::smem_u32(sm + L::OFF_K + (j & 1) * L::TILE);
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint64_t ad = tc::sdesc_sw128(q_base + (kk >> 2) * CP_HALF + (kk & 3) * 32, 16, 1024);
-          const uint64_t bd = tc::sdesc_sw128(k_base + (kk >> 2) * CP_HALF + (kk & 3) * 32, 16, 1024);
-          tc::mma_f16(tmem + (j & 1) * CP_N, ad, bd, id_s, kk > 0 ? 1u : 0u);
-        }
-        tc::tc_commit(&s_full[j & 1]);
-        tc::tc_commit(&k_empty[j & 1]);
-        if (j >= 1 && !issue_pv(j - 1)) ok = false;
+        conv_sync(); // every warp is done with rowoff of tile j
       }
-      if (ok && !issue_pv(ntiles - 1)) ok = false;
-      if (!ok) {
-        atomicExch(&g_cache_attn_prefill_status, tc::kTimeoutFull);
+      if (!ok && lane == 0 && !*abort_flag) {
+        atomicExch(&g_cache_attn_prefill_status, tc::kTimeoutEmpty);
         *abort_flag = 1;
       }
-      // TMEM is freed below: wait (bounded) until every issued MMA is done
-      tc::tc_commit(mma_done);
-      tc::mbar_wait(mma_done, 0);
-    }
+    } else {
+      // ------------------------------ MMA issuer --------------------------------
+      if (tc::elect_one()) {
+        const uint32_t id_s = tc::idesc(1, 0, 0, 0, 0, CP_M, CP_N);
+        const uint32_t id_o = tc::idesc(1, 0, 0, 0, 1, CP_M, DP);
+        const uint32_t q_base = tc::smem_u32(sm + L::OFF_Q);
+        bool ok = tc::mbar_wait(q_full, 0);
+        auto issue_pv = [&](int j) { // O (+)= P_j V_j, V read MN-major over the head's columns
+          if (!tc::mbar_wait(&p_full[j & 1], (j >> 1) & 1)) return false;
+          if (!tc::mbar_wait(&v_full[j & 1], (j >> 1) & 1)) return false;
+          tc::tc_fence_after();
+          const uint32_t p_col = tmem + (uint32_t)(j & 1) * CP_N;
+          const uint32_t v_base = tc::smem_u32(sm + L::OFF_V + (j & 1) * L::TILE);
+  #pragma unroll
+          for (int kk = 0; kk < CP_N / 16; ++kk) {
+            const uint64_t bd = tc::sdesc_sw128(v_base + kk * 16 * 128, CP_HALF, 1024);
+            tc::mma_f16_ts(tmem + CP_COL_O, p_col + kk * 8, bd, id_o, (j > 0 || kk > 0) ? 1u : 0u);
+          }
+          tc::tc_commit(&o_done[j & 1]);
+          tc::tc_commit(&v_empty[j & 1]);
+          return true;
+        };
+        for (int j = 0; ok && j < ntiles; ++j) {
+          if (*abort_flag || !tc::mbar_wait(&k_full[j & 1], (j >> 1) & 1)) {
+            ok = false;
+            break;
+          }
+          // S buffer j & 1 holds P_{j-2} until P.V of tile j - 2 is done
+          if (j >= 2 && !tc::mbar_wait(&o_done[j & 1], ((j - 2) >> 1) & 1)) {
+            ok = false;
+            break;
+          }
+          tc::tc_fence_after();
+          const uint32_t k_base = tc::smem_u32(sm + L::OFF_K + (j & 1) * L::TILE);
+  #pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk) {
+            const uint64_t ad = tc::sdesc_sw128(q_base + (kk >> 2) * CP_HALF + (kk & 3) * 32, 16, 1024);
+            const uint64_t bd = tc::sdesc_sw128(k_base + (kk >> 2) * CP_HALF + (kk & 3) * 32, 16, 1024);
+            tc::mma_f16(tmem + (j & 1) * CP_N, ad, bd, id_s, kk > 0 ? 1u : 0u);
+          }
+          tc::tc_commit(&s_full[j & 1]);
+          tc::tc_commit(&k_empty[j & 1]);
+          if (j >= 1 && !issue_pv(j - 1)) ok = false;
+        }
+        if (ok && !issue_pv(ntiles - 1)) ok = false;
+        if (!ok) {
+          atomicExch(&g_cache_attn_prefill_status, tc::kTimeoutFull);
+          *abort_flag = 1;
+        }
+        // TMEM is freed below: wait (bounded) until every issued MMA is done
+        tc::tc_commit(mma_done);
+        tc::mbar_wait(mma_done, 0);
+      }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CP_REG_SOFT));
     // ------------------------------ softmax warps -----------------------------
     // Warps w and w + 4 share TMEM lanes 32 (w % 4) .. + 31; each thread has one half of its row's
     // columns.  Control flow stays warp-uniform around the TMEM accesses, and every softmax warp
@@ -606,6 +608,7 @@ int cache_attn_prefill_launch(const CaArgs &a, bool f16, bool f8, cudaStream_t s
   g.qtiles = (a.S + g.np - 1) / g.np;
   g.hpacks = a.Hq / g.pk;
   g.scale_log2 = a.scale * kLog2E;
+  g.div_t = FastDiv((uint32_t)a.T);
   const unsigned grid = (unsigned)cache_attn_prefill_ctas(a);
   if (f16) return f8 ? cp_launch<__half, Fp8>(g, grid, st) : cp_launch<__half, Int8>(g, grid, st);
   return f8 ? cp_launch<__nv_bfloat16, Fp8>(g, grid, st) : cp_launch<__nv_bfloat16, Int8>(g, grid, st);
