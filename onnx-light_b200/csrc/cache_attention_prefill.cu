@@ -54,8 +54,8 @@ template <int DP> struct CpLayout {
   static constexpr uint32_t OFF_K = TILE, OFF_V = 3 * TILE; // two buffers each
   static constexpr uint32_t OFF_RED = 5 * TILE;             // [2][2][128] floats
   static constexpr uint32_t OFF_SC = OFF_RED + 2 * 2 * CP_M * 4;  // float4 [4 tiles][8 chunks]
-  static constexpr uint32_t OFF_ROW = OFF_SC + 4 * 8 * 16;        // int64 [2][128]: first code of a key's row, or -1
-  static constexpr uint32_t OFF_BAR = OFF_ROW + 2 * CP_N * 8;
+  static constexpr uint32_t OFF_ROW = OFF_SC + 4 * 8 * 16;        // int64 [4][128]: first code of a key's row, or -1
+  static constexpr uint32_t OFF_BAR = OFF_ROW + 4 * CP_N * 8;
   static constexpr int NBAR = 16;
   static constexpr size_t SMEM = OFF_BAR + NBAR * 8 + 16;
 };
@@ -173,41 +173,66 @@ __global__ void __launch_bounds__(CP_THREADS, 1) cache_attn_prefill(const CpArgs
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CP_REG_REST));
     if (warp >= CP_CONV) {
       // ------------------------------ converters --------------------------------
-      // The first 128 threads look after one key of each tile: the place of its codes goes to rowoff,
-      // two tiles deep, and every 16th key's page scales to sc, four deep (the softmax of a tile reads
-      // them while the converters are up to three tiles ahead).
+      // The first 128 threads look after one key of each tile: the place of its codes goes to rowoff
+      // and every 16th key's page scales to sc, both four tiles deep (a warp is at most one tile
+      // behind another, and the softmax of a tile reads sc while the converters are up to three
+      // ahead).  Page numbers are read two tiles ahead and scales one, so neither is waited for.
       const int ct = threadIdx.x - CP_CONV * 32, cw = warp - CP_CONV;
-      auto conv_sync = [] { asm volatile("bar.sync 2, %0;" ::"n"(CP_NCONV * 32) : "memory"); };
-      auto page_of = [&](int j, int r) -> int { // page of key r of tile j; -1: the sequence has no such key
-        if (j >= ntiles || r >= CP_N) return -1;
-        const int key = key0_of(j) + r;
+      // Barrier of the converters; true when `mine` holds for any of them.
+      auto conv_any = [](bool mine) {
+        int any;
+        asm volatile("{\n\t.reg .pred p, q;\n\t"
+                     "setp.ne.b32 p, %1, 0;\n\t"
+                     "barrier.cta.red.or.pred q, 2, %2, p;\n\t"
+                     "selp.b32 %0, 1, 0, q;\n\t}"
+                     : "=r"(any)
+                     : "r"((int)mine), "n"(CP_NCONV * 32)
+                     : "memory");
+        return any != 0;
+      };
+      struct Place {
+        int id; // page of the key; -1: the sequence has no such key
+        float ks, vs;
+      };
+      auto page_of = [&](int j) {
+        if (j >= ntiles || ct >= CP_N) return -1;
+        const int key = key0_of(j) + ct;
         return key < sp.total ? a.table[(int64_t)b * a.max_pages + g.div_t.div(key)] : -1;
       };
-      auto note = [&](int j, int r, int id) {
-        if (j >= ntiles || r >= CP_N) return;
-        const int key = key0_of(j) + r;
-        const bool has = key < sp.total, ok = has && id >= 0 && id < a.pages;
-        if (has && !ok) atomicExch(&g_cache_attn_prefill_range, 1);
-        const int64_t z = (int64_t)id * a.Hkv + kvh;
-        rowoff[(j & 1) * CP_N + r] = ok ? (z * a.T + (key - (int)g.div_t.div(key) * a.T)) * a.D : -1;
-        if (r % 16 == 0) {
-          float4 c = make_float4(0.0f, CP_LV_MIN, 0.0f, 0.0f);
-          if (ok) {
-            const float ks = a.ks[z] * g.scale_log2, vs = a.vs[z];
-            c.x = ks;
-            c.y = fmaxf(log2f(vs), CP_LV_MIN); // a NaN gives the bound
-            c.z = exp2f(-c.y);
-            // 1: scales of ordinary values; 2: the softmax looks at each score
-            const bool plain = ks > 0.0f && ks < INFINITY && fabsf(vs) < INFINITY;
-            c.w = plain ? 1.0f : 2.0f;
-            if (!(fabsf(vs) < INFINITY)) c.z = __uint_as_float(0x7fc00000u);
-          }
-          sc[(j & 3) * 8 + r / 16] = c;
+      auto scales_of = [&](int id) {
+        Place c{id, 0.0f, 0.0f};
+        if (ct % 16 == 0 && id >= 0 && id < a.pages) {
+          c.ks = a.ks[(int64_t)id * a.Hkv + kvh];
+          c.vs = a.vs[(int64_t)id * a.Hkv + kvh];
         }
+        return c;
+      };
+      // writes down tile j's place of this thread's key; whether its value scale is below 2^-60
+      auto note = [&](int j, const Place &c) {
+        if (j >= ntiles || ct >= CP_N) return false;
+        const int key = key0_of(j) + ct;
+        const bool has = key < sp.total, ok = has && c.id >= 0 && c.id < a.pages;
+        if (has && !ok) atomicExch(&g_cache_attn_prefill_range, 1);
+        rowoff[(j & 3) * CP_N + ct] =
+            ok ? (((int64_t)c.id * a.Hkv + kvh) * a.T + (key - (int)g.div_t.div(key) * a.T)) * a.D : -1;
+        if (ct % 16 != 0) return false;
+        float4 f = make_float4(0.0f, CP_LV_MIN, 0.0f, 0.0f);
+        if (ok) {
+          f.x = c.ks * g.scale_log2;
+          f.y = fmaxf(log2f(c.vs), CP_LV_MIN); // a NaN gives the bound
+          f.z = exp2f(-f.y);
+          // 1: scales of ordinary values; 2: the softmax looks at each score
+          f.w = f.x > 0.0f && f.x < INFINITY && fabsf(c.vs) < INFINITY ? 1.0f : 2.0f;
+          if (!(fabsf(c.vs) < INFINITY)) f.z = __uint_as_float(0x7fc00000u);
+        }
+        sc[(j & 3) * 8 + ct / 16] = f;
+        return ok && f.y <= CP_LV_MIN;
       };
       // 16-code units: lanes cover DP / 16 units of 512 / DP keys; a warp takes every seventh group
       constexpr int UPR = DP / 16, KPW = 32 / UPR, GROUPS = CP_N / KPW, MINE = (GROUPS + CP_NCONV - 1) / CP_NCONV;
-      const int u = lane % UPR, sub = lane / UPR;
+      // eight neighbouring lanes write four units of two rows: no bank is hit twice
+      const int u = DP == 64 ? lane & 3 : (lane & 3) | (lane >> 1 & 4);
+      const int sub = DP == 64 ? lane >> 2 : (lane >> 2 & 1) | (lane >> 4) * 2;
       const bool has_cols = u * 16 < a.D;
       uint4 kr[MINE], vr[MINE];
       auto load = [&](const uint8_t *pool, int j, uint4 (&r)[MINE]) {
@@ -216,13 +241,13 @@ __global__ void __launch_bounds__(CP_THREADS, 1) cache_attn_prefill(const CpArgs
           const int grp = cw + i * CP_NCONV;
           r[i] = make_uint4(0u, 0u, 0u, 0u);
           if (grp < GROUPS && has_cols) {
-            const int64_t off = rowoff[(j & 1) * CP_N + grp * KPW + sub];
+            const int64_t off = rowoff[(j & 3) * CP_N + grp * KPW + sub];
             if (off >= 0) r[i] = __ldg(reinterpret_cast<const uint4 *>(pool + off + u * 16));
           }
         }
       };
       // zero codes widen to zeros, so keys without a token and columns past D become zeros
-      auto store = [&](uint32_t base, int j, const uint4 (&r)[MINE], bool values) {
+      auto store = [&](uint32_t base, int j, const uint4 (&r)[MINE], bool tiny) {
   #pragma unroll
         for (int i = 0; i < MINE; ++i) {
           const int grp = cw + i * CP_NCONV, row = grp * KPW + sub;
@@ -231,17 +256,15 @@ __global__ void __launch_bounds__(CP_THREADS, 1) cache_attn_prefill(const CpArgs
             uint32_t h[8];
   #pragma unroll
             for (int q = 0; q < 4; ++q) widen4<Q>(w[q], h[2 * q], h[2 * q + 1]);
-            if (values) {
-              const float lv = sc[(j & 3) * 8 + row / 16].y;
-              if (lv <= CP_LV_MIN) { // a value scale below 2^-60: what 2^lv does not hold goes into the codes
-                const int64_t off = rowoff[(j & 1) * CP_N + row];
-                const float vs = off >= 0 ? a.vs[off / a.D / a.T] : 0.0f;
-                const float f = fabsf(vs) < INFINITY ? vs * exp2f(-CP_LV_MIN) : 0.0f;
-  #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                  const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&h[q]));
-                  h[q] = half2_of(v.x * f, v.y * f);
-                }
+            if (tiny && sc[(j & 3) * 8 + row / 16].y <= CP_LV_MIN) {
+              // a value scale below 2^-60: what 2^-60 does not hold goes into the codes
+              const int64_t off = rowoff[(j & 3) * CP_N + row];
+              const float vs = off >= 0 ? a.vs[off / a.D / a.T] : 0.0f;
+              const float f = fabsf(vs) < INFINITY ? vs * exp2f(-CP_LV_MIN) : 0.0f;
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&h[q]));
+                h[q] = half2_of(v.x * f, v.y * f);
               }
             }
             uint8_t *p = sm + base + (u >> 2) * CP_HALF + row * 128;
@@ -251,17 +274,17 @@ __global__ void __launch_bounds__(CP_THREADS, 1) cache_attn_prefill(const CpArgs
           }
         }
       };
-      note(0, ct, page_of(0, ct));
-      int id = page_of(1, ct);
-      conv_sync();
+      const int id0 = page_of(0);
+      int id = page_of(1);
+      bool tiny = conv_any(note(0, scales_of(id0)));
+      Place next = scales_of(id);
       load(a.k, 0, kr);
       bool ok = true;
       for (int j = 0; j < ntiles; ++j) {
         const int s = j & 1;
         load(a.v, j, vr);
-        // the next tile's places (the buffer's last reader was this warp group's V of tile j - 1)
-        note(j + 1, ct, id);
-        id = page_of(j + 2, ct);
+        const bool mine = note(j + 1, next);
+        id = page_of(j + 2);
         if (ok && (*abort_flag || (j >= 2 && !tc::mbar_wait(&k_empty[s], ((j - 2) >> 1) & 1)))) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
@@ -270,17 +293,18 @@ __global__ void __launch_bounds__(CP_THREADS, 1) cache_attn_prefill(const CpArgs
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(&k_full[s]);
         }
-        conv_sync(); // rowoff and sc of tile j + 1 are written
+        const bool tiny_next = conv_any(mine); // rowoff and sc of tile j + 1 are written
         if (j + 1 < ntiles) load(a.k, j + 1, kr);
         if (ok && (*abort_flag || (j >= 2 && !tc::mbar_wait(&v_empty[s], ((j - 2) >> 1) & 1)))) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
-          store(L::OFF_V + s * L::TILE, j, vr, true);
+          store(L::OFF_V + s * L::TILE, j, vr, tiny);
           tc::fence_proxy_async();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(&v_full[s]);
         }
-        conv_sync(); // every warp is done with rowoff of tile j
+        next = scales_of(id);
+        tiny = tiny_next;
       }
       if (!ok && lane == 0 && !*abort_flag) {
         atomicExch(&g_cache_attn_prefill_status, tc::kTimeoutEmpty);
@@ -339,7 +363,7 @@ __global__ void __launch_bounds__(CP_THREADS, 1) cache_attn_prefill(const CpArgs
         tc::tc_commit(mma_done);
         tc::mbar_wait(mma_done, 0);
       }
-  }
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CP_REG_SOFT));
     // ------------------------------ softmax warps -----------------------------
