@@ -6,9 +6,10 @@
 // One CTA owns 128 query rows -- pk heads of one GQA group (pk the largest power of two up to 8 that
 // divides the group) x 128 / pk positions -- and walks the 128-key tiles that any of them sees (the
 // sinks' tiles, then the window's up to the diagonal):
-//   warps 9-15 (converters) read the tile's codes from their pages, 16 bytes a lane, widen them to
-//              FLOAT16 (exact for both code types) and write the 128-byte-swizzled K and V
-//              operands, two buffers each; rows that hold no token become zeros;
+//   warp 9     (pages) looks up the tiles' pages and scales ahead of use and brings the codes by TMA,
+//              one box per run of a page's tokens, K and V through two buffers each;
+//   warps 10-15 (converters) widen the codes to FLOAT16 (exact for both code types) and write the
+//              128-byte-swizzled K and V operands, two buffers each; rows without a token become zeros;
 //   warp 8     (MMA) issues S = Q K^T into one of two TMEM buffers and O += P V with P read from TMEM;
 //   warps 0-7  (softmax) two threads per query row, one per half of the columns.
 // Scales never touch an element: within 16 keys of one page the key scale is part of the exponent's
@@ -37,12 +38,13 @@ namespace {
 using namespace q8;
 
 constexpr int CP_M = 128, CP_N = 128;             // query rows, keys per tile
-constexpr int CP_SOFT = 8, CP_MMA = 8, CP_CONV = 9, CP_NCONV = 7;
-// Registers: 16 warps start with 128 each; the two softmax warpgroups take 168, the other two keep
-// 88 (2 x 168 + 2 x 88 = 4 x 128).
-constexpr int CP_REG_SOFT = 168, CP_REG_REST = 88;
+constexpr int CP_SOFT = 8, CP_MMA = 8, CP_PAGES = 9, CP_CONV = 10, CP_NCONV = 6;
+// Registers: 16 warps start with 128 each; the two softmax warpgroups take 160, the other two keep
+// 96 (2 x 160 + 2 x 96 = 4 x 128).
+constexpr int CP_REG_SOFT = 160, CP_REG_REST = 96;
 constexpr int CP_THREADS = (CP_CONV + CP_NCONV) * 32;
 constexpr uint32_t CP_HALF = 128 * 128;           // [128 rows][64 FLOAT16]: 16 KB
+constexpr uint32_t CP_RAW = 128 * 128;            // a tile's codes, 128 bytes a key
 constexpr uint32_t CP_TMEM_COLS = 512, CP_COL_O = 256;
 constexpr float CP_TOP = 15.0f, CP_BASE = 7.0f;   // log2 of the largest p', and after a move of m
 constexpr float CP_LV_MIN = -60.0f;
@@ -52,11 +54,12 @@ template <int DP> struct CpLayout {
   static constexpr uint32_t TILE = NH * CP_HALF;  // a K or V operand
   static constexpr uint32_t OFF_Q = 0;
   static constexpr uint32_t OFF_K = TILE, OFF_V = 3 * TILE; // two buffers each
-  static constexpr uint32_t OFF_RED = 5 * TILE;             // [2][2][128] floats
-  static constexpr uint32_t OFF_SC = OFF_RED + 2 * 2 * CP_M * 4;  // float4 [4 tiles][8 chunks]
-  static constexpr uint32_t OFF_ROW = OFF_SC + 4 * 8 * 16;        // int64 [4][128]: first code of a key's row, or -1
-  static constexpr uint32_t OFF_BAR = OFF_ROW + 4 * CP_N * 8;
-  static constexpr int NBAR = 16;
+  static constexpr uint32_t OFF_RAW = 5 * TILE;             // codes [128][128 B]: K, K, V, V
+  static constexpr uint32_t OFF_RED = OFF_RAW + 4 * CP_RAW;  // float [2][2][128]
+  static constexpr uint32_t OFF_SC = OFF_RED + 2 * 2 * CP_M * 4; // float4 [4 tiles][8 runs of 16 keys]
+  static constexpr uint32_t OFF_FAC = OFF_SC + 4 * 8 * 16;       // float [4][8], then int [4]
+  static constexpr uint32_t OFF_BAR = OFF_FAC + 4 * 8 * 4 + 16;
+  static constexpr int NBAR = 24;
   static constexpr size_t SMEM = OFF_BAR + NBAR * 8 + 16;
 };
 
@@ -65,6 +68,7 @@ struct CpArgs {
   int qtiles, pk, np, hpacks;
   float scale_log2;
   FastDiv div_t; // by the page size
+  int chunk;     // keys per TMA box: a power of two, 16 to 128, that divides the page
 };
 
 // Four codes -> two FLOAT16 pairs, exactly.
@@ -93,7 +97,9 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
 }
 
 template <typename T, typename Q, int DP>
-__global__ void __launch_bounds__(CP_THREADS, 1) cache_attn_prefill(const CpArgs g) {
+__global__ void __launch_bounds__(CP_THREADS, 1)
+    cache_attn_prefill(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                       const CpArgs g) {
   using L = CpLayout<DP>;
   extern __shared__ __align__(1024) uint8_t sm[];
   if (tc::smem_u32(sm) & 1023u) { // the operands need a 1024-byte aligned base
@@ -104,7 +110,8 @@ __global__ void __launch_bounds__(CP_THREADS, 1) cache_attn_prefill(const CpArgs
   uint64_t *bars = reinterpret_cast<uint64_t *>(sm + L::OFF_BAR);
   float *red = reinterpret_cast<float *>(sm + L::OFF_RED);
   float4 *sc = reinterpret_cast<float4 *>(sm + L::OFF_SC);
-  int64_t *rowoff = reinterpret_cast<int64_t *>(sm + L::OFF_ROW);
+  float *fac = reinterpret_cast<float *>(sm + L::OFF_FAC);           // of value scales below 2^-60
+  volatile int *look = reinterpret_cast<volatile int *>(sm + L::OFF_FAC + 4 * 8 * 4); // [4] per tile: what converters check
   uint64_t *q_full = bars;       // 1
   uint64_t *k_full = bars + 1;   // 2
   uint64_t *k_empty = bars + 3;  // 2: S of the buffer's tile done
@@ -114,6 +121,8 @@ __global__ void __launch_bounds__(CP_THREADS, 1) cache_attn_prefill(const CpArgs
   uint64_t *p_full = bars + 11;  // 2
   uint64_t *o_done = bars + 13;  // 2
   uint64_t *mma_done = bars + 15;
+  uint64_t *raw_full = bars + 16;  // 4: the codes of K (0, 1) and V (2, 3) landed
+  uint64_t *raw_empty = bars + 20; // 4: converted
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + L::NBAR);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
@@ -156,6 +165,10 @@ __global__ void __launch_bounds__(CP_THREADS, 1) cache_attn_prefill(const CpArgs
       tc::mbar_init(&p_full[i], CP_SOFT);
       tc::mbar_init(&o_done[i], 1);
     }
+    for (int i = 0; i < 4; ++i) {
+      tc::mbar_init(&raw_full[i], 1);
+      tc::mbar_init(&raw_empty[i], CP_NCONV);
+    }
     tc::mbar_init(mma_done, 1);
     *abort_flag = 0;
     tc::fence_barrier_init();
@@ -173,94 +186,39 @@ __global__ void __launch_bounds__(CP_THREADS, 1) cache_attn_prefill(const CpArgs
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CP_REG_REST));
     if (warp >= CP_CONV) {
       // ------------------------------ converters --------------------------------
-      // The first 128 threads look after one key of each tile: the place of its codes goes to rowoff
-      // and every 16th key's page scales to sc, both four tiles deep (a warp is at most one tile
-      // behind another, and the softmax of a tile reads sc while the converters are up to three
-      // ahead).  Page numbers are read two tiles ahead and scales one, so neither is waited for.
-      const int ct = threadIdx.x - CP_CONV * 32, cw = warp - CP_CONV;
-      // Barrier of the converters; true when `mine` holds for any of them.
-      auto conv_any = [](bool mine) {
-        int any;
-        asm volatile("{\n\t.reg .pred p, q;\n\t"
-                     "setp.ne.b32 p, %1, 0;\n\t"
-                     "barrier.cta.red.or.pred q, 2, %2, p;\n\t"
-                     "selp.b32 %0, 1, 0, q;\n\t}"
-                     : "=r"(any)
-                     : "r"((int)mine), "n"(CP_NCONV * 32)
-                     : "memory");
-        return any != 0;
-      };
-      struct Place {
-        int id; // page of the key; -1: the sequence has no such key
-        float ks, vs;
-      };
-      auto page_of = [&](int j) {
-        if (j >= ntiles || ct >= CP_N) return -1;
-        const int key = key0_of(j) + ct;
-        return key < sp.total ? a.table[(int64_t)b * a.max_pages + g.div_t.div(key)] : -1;
-      };
-      auto scales_of = [&](int id) {
-        Place c{id, 0.0f, 0.0f};
-        if (ct % 16 == 0 && id >= 0 && id < a.pages) {
-          c.ks = a.ks[(int64_t)id * a.Hkv + kvh];
-          c.vs = a.vs[(int64_t)id * a.Hkv + kvh];
-        }
-        return c;
-      };
-      // writes down tile j's place of this thread's key; whether its value scale is below 2^-60
-      auto note = [&](int j, const Place &c) {
-        if (j >= ntiles || ct >= CP_N) return false;
-        const int key = key0_of(j) + ct;
-        const bool has = key < sp.total, ok = has && c.id >= 0 && c.id < a.pages;
-        if (has && !ok) atomicExch(&g_cache_attn_prefill_range, 1);
-        rowoff[(j & 3) * CP_N + ct] =
-            ok ? (((int64_t)c.id * a.Hkv + kvh) * a.T + (key - (int)g.div_t.div(key) * a.T)) * a.D : -1;
-        if (ct % 16 != 0) return false;
-        float4 f = make_float4(0.0f, CP_LV_MIN, 0.0f, 0.0f);
-        if (ok) {
-          f.x = c.ks * g.scale_log2;
-          f.y = fmaxf(log2f(c.vs), CP_LV_MIN); // a NaN gives the bound
-          f.z = exp2f(-f.y);
-          // 1: scales of ordinary values; 2: the softmax looks at each score
-          f.w = f.x > 0.0f && f.x < INFINITY && fabsf(c.vs) < INFINITY ? 1.0f : 2.0f;
-          if (!(fabsf(c.vs) < INFINITY)) f.z = __uint_as_float(0x7fc00000u);
-        }
-        sc[(j & 3) * 8 + ct / 16] = f;
-        return ok && f.y <= CP_LV_MIN;
-      };
-      // 16-code units: lanes cover DP / 16 units of 512 / DP keys; a warp takes every seventh group
+      // 16-code units: lanes cover DP / 16 units of 512 / DP keys; a warp takes every sixth group.
+      // Eight neighbouring lanes have four units of two rows, so no bank is hit twice.
+      const int cw = warp - CP_CONV;
       constexpr int UPR = DP / 16, KPW = 32 / UPR, GROUPS = CP_N / KPW, MINE = (GROUPS + CP_NCONV - 1) / CP_NCONV;
-      // eight neighbouring lanes write four units of two rows: no bank is hit twice
       const int u = DP == 64 ? lane & 3 : (lane & 3) | (lane >> 1 & 4);
       const int sub = DP == 64 ? lane >> 2 : (lane >> 2 & 1) | (lane >> 4) * 2;
-      const bool has_cols = u * 16 < a.D;
-      uint4 kr[MINE], vr[MINE];
-      auto load = [&](const uint8_t *pool, int j, uint4 (&r)[MINE]) {
-  #pragma unroll
+      auto widen = [&](uint32_t raw, uint32_t base, int j, bool values) {
+        const int check = look[j & 3];
+        uint4 r[MINE];
+#pragma unroll
         for (int i = 0; i < MINE; ++i) {
-          const int grp = cw + i * CP_NCONV;
-          r[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (grp < GROUPS && has_cols) {
-            const int64_t off = rowoff[(j & 3) * CP_N + grp * KPW + sub];
-            if (off >= 0) r[i] = __ldg(reinterpret_cast<const uint4 *>(pool + off + u * 16));
+          const int row = (cw + i * CP_NCONV) * KPW + sub;
+          if (row < CP_N) r[i] = *reinterpret_cast<const uint4 *>(sm + raw + row * 128 + ((u ^ (row & 7)) << 4));
+        }
+        if (check) { // zero codes widen to zeros
+#pragma unroll
+          for (int i = 0; i < MINE; ++i) {
+            const int row = (cw + i * CP_NCONV) * KPW + sub;
+            if (row < CP_N && (key0_of(j) + row >= sp.total || sc[(j & 3) * 8 + row / 16].w == 0.0f))
+              r[i] = make_uint4(0u, 0u, 0u, 0u);
           }
         }
-      };
-      // zero codes widen to zeros, so keys without a token and columns past D become zeros
-      auto store = [&](uint32_t base, int j, const uint4 (&r)[MINE], bool tiny) {
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < MINE; ++i) {
-          const int grp = cw + i * CP_NCONV, row = grp * KPW + sub;
-          if (grp < GROUPS) {
+          const int row = (cw + i * CP_NCONV) * KPW + sub;
+          if (row < CP_N) {
             const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
             uint32_t h[8];
-  #pragma unroll
+#pragma unroll
             for (int q = 0; q < 4; ++q) widen4<Q>(w[q], h[2 * q], h[2 * q + 1]);
-            if (tiny && sc[(j & 3) * 8 + row / 16].y <= CP_LV_MIN) {
-              // a value scale below 2^-60: what 2^-60 does not hold goes into the codes
-              const int64_t off = rowoff[(j & 3) * CP_N + row];
-              const float vs = off >= 0 ? a.vs[off / a.D / a.T] : 0.0f;
-              const float f = fabsf(vs) < INFINITY ? vs * exp2f(-CP_LV_MIN) : 0.0f;
+            if (values && (check & 2)) {
+              // value scales below 2^-60: what 2^-60 does not hold goes into the codes
+              const float f = fac[(j & 3) * 8 + row / 16];
 #pragma unroll
               for (int q = 0; q < 8; ++q) {
                 const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&h[q]));
@@ -273,42 +231,125 @@ __global__ void __launch_bounds__(CP_THREADS, 1) cache_attn_prefill(const CpArgs
             *reinterpret_cast<uint4 *>(p + (((c + 1) ^ (row & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
           }
         }
+        tc::fence_proxy_async();
+        __syncwarp();
       };
-      const int id0 = page_of(0);
-      int id = page_of(1);
-      bool tiny = conv_any(note(0, scales_of(id0)));
-      Place next = scales_of(id);
-      load(a.k, 0, kr);
       bool ok = true;
-      for (int j = 0; j < ntiles; ++j) {
+      for (int j = 0; ok && j < ntiles; ++j) {
         const int s = j & 1;
-        load(a.v, j, vr);
-        const bool mine = note(j + 1, next);
-        id = page_of(j + 2);
-        if (ok && (*abort_flag || (j >= 2 && !tc::mbar_wait(&k_empty[s], ((j - 2) >> 1) & 1)))) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok) {
-          store(L::OFF_K + s * L::TILE, j, kr, false);
-          tc::fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&k_full[s]);
+        const uint32_t ph = (j >> 1) & 1;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          uint64_t *empty = v ? v_empty : k_empty;
+          ok = ok && !*abort_flag && tc::mbar_wait(&raw_full[2 * v + s], ph) &&
+               (j < 2 || tc::mbar_wait(&empty[s], ph ^ 1));
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          widen(L::OFF_RAW + (2 * v + s) * CP_RAW, (v ? L::OFF_V : L::OFF_K) + s * L::TILE, j, v == 1);
+          if (lane == 0) {
+            tc::mbar_arrive(&raw_empty[2 * v + s]);
+            tc::mbar_arrive(v ? &v_full[s] : &k_full[s]);
+          }
         }
-        const bool tiny_next = conv_any(mine); // rowoff and sc of tile j + 1 are written
-        if (j + 1 < ntiles) load(a.k, j + 1, kr);
-        if (ok && (*abort_flag || (j >= 2 && !tc::mbar_wait(&v_empty[s], ((j - 2) >> 1) & 1)))) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok) {
-          store(L::OFF_V + s * L::TILE, j, vr, tiny);
-          tc::fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&v_full[s]);
-        }
-        next = scales_of(id);
-        tiny = tiny_next;
       }
-      if (!ok && lane == 0 && !*abort_flag) {
+      if (!ok && lane == 0) {
         atomicExch(&g_cache_attn_prefill_status, tc::kTimeoutEmpty);
         *abort_flag = 1;
+      }
+    } else if (warp == CP_PAGES) {
+      // ------------------------------ pages --------------------------------------
+      // Lane (my, ch) has box ch of tile my of each batch of `per` tiles; page numbers are read two
+      // batches ahead and scales one.  A tile's scales go to sc, four tiles deep: both buffers of tile
+      // j - 2 are converted before tile j is written, so P.V of tile j - 4 is done, and its softmax.
+      const int nch = CP_N / g.chunk, per = 32 / nch, my = lane / nch, ch = lane % nch;
+      const uint32_t box_bytes = (uint32_t)g.chunk * 128;
+      if (lane == 0) {
+        tc::prefetch_tensormap(&map_k);
+        tc::prefetch_tensormap(&map_v);
+      }
+      struct Box {
+        int id, row; // page (-1: no token of the sequence), first row in it
+      };
+      auto find = [&](int j) {
+        Box x{-1, 0};
+        if (j < ntiles) {
+          const int key = key0_of(j) + ch * g.chunk;
+          if (key < sp.total) {
+            const int page = (int)g.div_t.div(key);
+            x.id = a.table[(int64_t)b * a.max_pages + page];
+            x.row = key - page * a.T;
+            if (x.id < 0 || x.id >= a.pages) {
+              atomicExch(&g_cache_attn_prefill_range, 1);
+              x.id = -1;
+            }
+          }
+        }
+        return x;
+      };
+      auto scales = [&](const Box &x) {
+        return x.id >= 0 ? make_float2(a.ks[x.id * a.Hkv + kvh], a.vs[x.id * a.Hkv + kvh]) : make_float2(0.0f, 0.0f);
+      };
+      bool ok = true;
+      int issued = 0;
+      Box x0 = find(my), x1 = find(per + my);
+      float2 s0 = scales(x0);
+      for (int j0 = 0; ok && j0 < ntiles; j0 += per) {
+        const float2 s1 = scales(x1);
+        const Box x2 = find(j0 + 2 * per + my);
+        float4 f = make_float4(0.0f, CP_LV_MIN, 0.0f, 0.0f);
+        if (x0.id >= 0) {
+          f.x = s0.x * g.scale_log2;
+          f.y = fmaxf(log2f(s0.y), CP_LV_MIN); // a NaN gives the bound
+          f.z = exp2f(-f.y);
+          // 1: scales of ordinary values; 2: the softmax looks at each score
+          f.w = f.x > 0.0f && f.x < INFINITY && fabsf(s0.y) < INFINITY ? 1.0f : 2.0f;
+          if (!(fabsf(s0.y) < INFINITY)) f.z = __uint_as_float(0x7fc00000u);
+        }
+        const bool tiny = x0.id >= 0 && f.y <= CP_LV_MIN;
+        const bool holes = x0.id < 0 || key0_of(min(j0 + my, ntiles - 1)) + (ch + 1) * g.chunk > sp.total;
+        const uint32_t tinies = __ballot_sync(0xffffffffu, tiny), holed = __ballot_sync(0xffffffffu, holes);
+        const uint32_t have = __ballot_sync(0xffffffffu, x0.id >= 0);
+        for (int k = 0; ok && k < per && j0 + k < ntiles; ++k) {
+          const int j = j0 + k, s = j & 1;
+          if (j >= 2) {
+            ok = tc::mbar_wait(&raw_empty[s], ((j >> 1) - 1) & 1) && tc::mbar_wait(&raw_empty[2 + s], ((j >> 1) - 1) & 1);
+          }
+          ok = __all_sync(0xffffffffu, ok && !*abort_flag);
+          if (!ok) break;
+          const uint32_t bits = (nch == 32 ? 0xffffffffu : (1u << nch) - 1u) << (k * nch);
+          const uint32_t bytes = (uint32_t)__popc(have & bits) * box_bytes;
+          if (my == k) {
+            for (int e = 0; e < g.chunk / 16; ++e) {
+              sc[(j & 3) * 8 + ch * (g.chunk / 16) + e] = f;
+              fac[(j & 3) * 8 + ch * (g.chunk / 16) + e] = tiny && fabsf(s0.y) < INFINITY ? s0.y * exp2f(-CP_LV_MIN) : tiny ? 0.0f : 1.0f;
+            }
+          }
+          if (lane == 0) look[j & 3] = ((holed & bits) ? 1 : 0) | ((tinies & bits) ? 2 : 0);
+          __syncwarp();
+          if (lane == 0) {
+            tc::mbar_expect_tx(&raw_full[s], bytes);
+            tc::mbar_expect_tx(&raw_full[2 + s], bytes);
+          }
+          __syncwarp();
+          if (my == k && x0.id >= 0) {
+            const int z = x0.id * a.Hkv + kvh;
+            tc::tma_load_3d(sm + L::OFF_RAW + s * CP_RAW + ch * box_bytes, &map_k, &raw_full[s], 0, x0.row, z);
+            tc::tma_load_3d(sm + L::OFF_RAW + (2 + s) * CP_RAW + ch * box_bytes, &map_v, &raw_full[2 + s], 0, x0.row, z);
+          }
+          issued = j + 1;
+        }
+        x0 = x1;
+        x1 = x2;
+        s0 = s1;
+      }
+      if (!ok && lane == 0) {
+        atomicExch(&g_cache_attn_prefill_status, tc::kTimeoutEmpty);
+        *abort_flag = 1;
+      }
+      // no copy may land once the CTA has left: wait (bounded) for the last fills of both buffers
+      for (int j = max(0, issued - 2); j < issued; ++j) {
+        tc::mbar_wait(&raw_full[j & 1], (j >> 1) & 1);
+        tc::mbar_wait(&raw_full[2 + (j & 1)], (j >> 1) & 1);
       }
     } else {
       // ------------------------------ MMA issuer --------------------------------
@@ -587,15 +628,16 @@ int cp_pk(int group) { // heads per CTA
   return pk;
 }
 
-template <typename T, typename Q> int cp_launch(const CpArgs &g, unsigned grid, cudaStream_t st) {
+template <typename T, typename Q>
+int cp_launch(const CUtensorMap &mk, const CUtensorMap &mv, const CpArgs &g, unsigned grid, cudaStream_t st) {
   if (g.c.D <= 64) {
     auto kern = cache_attn_prefill<T, Q, 64>;
     B2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)CpLayout<64>::SMEM));
-    kern<<<grid, CP_THREADS, CpLayout<64>::SMEM, st>>>(g);
+    kern<<<grid, CP_THREADS, CpLayout<64>::SMEM, st>>>(mk, mv, g);
   } else {
     auto kern = cache_attn_prefill<T, Q, 128>;
     B2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)CpLayout<128>::SMEM));
-    kern<<<grid, CP_THREADS, CpLayout<128>::SMEM, st>>>(g);
+    kern<<<grid, CP_THREADS, CpLayout<128>::SMEM, st>>>(mk, mv, g);
   }
   B2_LAUNCH_CHECK();
   return B2_OK;
@@ -621,7 +663,7 @@ int64_t cache_attn_prefill_ctas(const CaArgs &a) {
 
 bool cache_attn_prefill_eligible(const CaArgs &a) {
   return a.D % 16 == 0 && a.D <= 128 && a.T % 16 == 0 && aligned(a.q, 16) && aligned(a.y, 16) && aligned(a.k, 16) &&
-         aligned(a.v, 16) && a.q_h % 8 == 0 && a.q_s % 8 == 0 && cache_attn_prefill_ctas(a) < ((int64_t)1 << 31);
+         aligned(a.v, 16) && a.pages > 0 && a.q_h % 8 == 0 && a.q_s % 8 == 0 && cache_attn_prefill_ctas(a) < ((int64_t)1 << 31);
 }
 
 int cache_attn_prefill_launch(const CaArgs &a, bool f16, bool f8, cudaStream_t st) {
@@ -633,9 +675,17 @@ int cache_attn_prefill_launch(const CaArgs &a, bool f16, bool f8, cudaStream_t s
   g.hpacks = a.Hq / g.pk;
   g.scale_log2 = a.scale * kLog2E;
   g.div_t = FastDiv((uint32_t)a.T);
+  g.chunk = a.T % 128 == 0 ? 128 : a.T % 64 == 0 ? 64 : a.T % 32 == 0 ? 32 : 16;
   const unsigned grid = (unsigned)cache_attn_prefill_ctas(a);
-  if (f16) return f8 ? cp_launch<__half, Fp8>(g, grid, st) : cp_launch<__half, Int8>(g, grid, st);
-  return f8 ? cp_launch<__nv_bfloat16, Fp8>(g, grid, st) : cp_launch<__nv_bfloat16, Int8>(g, grid, st);
+  // [pages * Hkv][T][D] codes; columns past D read as zeros
+  CUtensorMap mk, mv;
+  const uint64_t dims[3] = {(uint64_t)a.D, (uint64_t)a.T, (uint64_t)a.pages * a.Hkv};
+  const uint64_t strides[2] = {(uint64_t)a.D, (uint64_t)a.T * a.D};
+  const uint32_t box[3] = {128, (uint32_t)g.chunk, 1};
+  if (int rc = make_tensor_map(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  if (int rc = make_tensor_map(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  if (f16) return f8 ? cp_launch<__half, Fp8>(mk, mv, g, grid, st) : cp_launch<__half, Int8>(mk, mv, g, grid, st);
+  return f8 ? cp_launch<__nv_bfloat16, Fp8>(mk, mv, g, grid, st) : cp_launch<__nv_bfloat16, Int8>(mk, mv, g, grid, st);
 }
 
 int status_read_cache_attn_prefill(int reset) { return cp_read(reset, g_cache_attn_prefill_status); }
