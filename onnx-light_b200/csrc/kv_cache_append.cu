@@ -82,19 +82,11 @@ __global__ void __launch_bounds__(KA_THREADS) kv_cache_append_kernel(const KaArg
       else held[k].zero();
     }
 #pragma unroll
-    for (int k = 0; k < KA_HELD; ++k) {
-      float f[8];
-      held[k].get(f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = max(m, mag(f[e]));
-    }
+    for (int k = 0; k < KA_HELD; ++k) m = max(m, mag8(held[k]));
     for (int v = threadIdx.x + KA_HELD * KA_THREADS; v < nv; v += KA_THREADS) {
       Raw8<T> x;
       x.load(src + at(v));
-      float f[8];
-      x.get(f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = max(m, mag(f[e]));
+      m = max(m, mag8(x));
     }
   } else {
     for (int v = threadIdx.x; v < nv; v += KA_THREADS) m = max(m, mag(ld1<T>(src, at(v))));
@@ -114,11 +106,11 @@ __global__ void __launch_bounds__(KA_THREADS) kv_cache_append_kernel(const KaArg
   // ---- the new codes ----
   dst += (int64_t)older * a.D;
   if constexpr (VEC) {
+    const Divisor by(s);
     auto put = [&](int v, const Raw8<T> &x) {
       float f[8];
       x.get(f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = __fdiv_rn(f[e], s);
+      by.divide(f);
       *reinterpret_cast<uint2 *>(dst + (int64_t)v * 8) = enc8<Q>(f);
     };
 #pragma unroll

@@ -32,28 +32,54 @@ template <> struct Code<Fp8> {
   static __device__ __forceinline__ float dec(uint32_t c) { return dec_f8e4m3fn(c); }
 };
 
-// Eight values -> eight code bytes, the first value in the lowest byte.
+// Eight finite values of at most kMax (and a rounding) -> eight code bytes, the first value in the
+// lowest byte.
 template <typename Q> __device__ __forceinline__ uint2 enc8(const float (&v)[8]) {
   uint2 r;
   if constexpr (std::is_same<Q, Fp8>::value) {
     uint32_t h[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = make_float2(v[2 * i] == v[2 * i] ? v[2 * i] : 0.0f,
-                                   v[2 * i + 1] == v[2 * i + 1] ? v[2 * i + 1] : 0.0f);
-      h[i] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
-    }
+    for (int i = 0; i < 4; ++i)
+      h[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
     r.x = h[0] | (h[1] << 16);
     r.y = h[2] | (h[3] << 16);
   } else {
+    // adding 1.5 * 2^23 rounds to nearest even and leaves the integer in the low bits
     uint32_t c[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = Code<Q>::enc(v[i]);
-    r.x = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
-    r.y = c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24);
+    for (int i = 0; i < 8; ++i) c[i] = __float_as_uint(v[i] + 12582912.0f);
+    r.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    r.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
   }
   return r;
 }
+
+// Division of many values by one scale, correctly rounded: with inv the correctly rounded 1 / s,
+// q = x inv is within an ulp or two, x - q s is exact in one FMA, and q + (x - q s) inv rounds to the
+// nearest quotient (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
+// processor", 1990, theorem on division by a correctly rounded reciprocal).  That needs s and inv
+// well inside the normal range; other scales take the division itself, and a scale that is 0, infinite
+// or not a number gives zeros, the code of such a group.
+struct Divisor {
+  float s, inv;
+  int kind; // 0 zeros, 1 products, 2 divisions
+  __device__ __forceinline__ explicit Divisor(float scale) : s(scale) {
+    kind = !(scale > 0.0f && scale < INFINITY) ? 0 : scale > 1e-30f && scale < 1e30f ? 1 : 2;
+    inv = kind == 1 ? __frcp_rn(scale) : 0.0f;
+  }
+  __device__ __forceinline__ void divide(float (&v)[8]) const {
+    if (kind == 1) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float q = v[e] * inv;
+        v[e] = fmaf(fmaf(-q, s, v[e]), inv, q);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = kind == 0 ? 0.0f : __fdiv_rn(v[e], s);
+    }
+  }
+};
 
 // Eight consecutive FLOAT16 / BFLOAT16 / FLOAT values as loaded (16-byte aligned).
 template <typename T> struct Raw8 {
@@ -130,6 +156,25 @@ __device__ __forceinline__ uint32_t block_max(uint32_t m, uint32_t *red) {
   const uint32_t n = blockDim.x >> 5;
   m = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < n ? red[threadIdx.x & 31] : 0u);
   return m;
+}
+
+// The largest magnitude of eight values as loaded, as mag() gives it.
+template <typename T> __device__ __forceinline__ uint32_t mag8(const Raw8<T> &x) {
+  if constexpr (std::is_same<T, float>::value) {
+    float f[8];
+    x.get(f);
+    uint32_t m = 0u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, mag(f[e]));
+    return m;
+  } else {
+    // 16-bit magnitudes order like unsigned integers, every NaN above infinity
+    const uint32_t m = __vmaxu2(__vmaxu2(x.a.x & 0x7fff7fffu, x.a.y & 0x7fff7fffu),
+                                __vmaxu2(x.a.z & 0x7fff7fffu, x.a.w & 0x7fff7fffu));
+    const uint32_t h = max(m & 0xffffu, m >> 16);
+    if constexpr (std::is_same<T, __half>::value) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+    else return h << 16;
+  }
 }
 
 inline bool is_q8(int dt) { return dt == kInt8 || dt == kF8E4M3FN; }

@@ -139,8 +139,7 @@ __global__ void __launch_bounds__(1024) rms_norm_q_vec(const RnqArgs a) {
   for (int k = 0; k < KV; ++k) {
     const int v = tid + k * nt;
     if (v < nv) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) h[k][e] = __fdiv_rn(h[k][e], s[k]);
+      Divisor(s[k]).divide(h[k]);
       *reinterpret_cast<uint2 *>(a.y + base + 8 * v) = enc8<Q>(h[k]);
     }
   }
