@@ -56,24 +56,17 @@ __global__ void __launch_bounds__(KA_THREADS) kv_cache_append_kernel(const KaArg
     if (bad && threadIdx.x == 0) atomicExch(&g_cache_append_status, 1);
     return;
   }
+  // The page number and the new values are read together: neither needs the other.
   const int64_t id = a.table[(int64_t)b * a.max_pages + page];
-  if (id < 0 || id >= a.pages) bad = true;
-  if (bad && threadIdx.x == 0) atomicExch(&g_cache_append_status, 1);
-  if (id < 0 || id >= a.pages) return;
   const int older = (int)(lo - page * a.T), rows = (int)(hi - lo);
-  float *sp = a.scale[side] + id * a.H + h;
-  uint8_t *dst = a.pool[side] + (id * a.H + h) * (int64_t)a.T * a.D;
   const T *src = static_cast<const T *>(a.src[side]) + (int64_t)b * a.s_b + (int64_t)h * a.s_h +
                  (lo - past) * a.s_s;
-  const float before = older ? *sp : 0.0f;
-  // ---- the largest magnitude of the new values ----
-  Raw8<T> held[KA_HELD];
-  uint32_t m = 0u;
   const int dv = VEC ? a.D >> 3 : a.D, nv = rows * dv;
   auto at = [&](int v) { // element offset of vector (or value) v of the new rows
     const int r = v / dv;
     return (int64_t)r * a.s_s + (int64_t)(v - r * dv) * (VEC ? 8 : 1);
   };
+  Raw8<T> held[KA_HELD];
   if constexpr (VEC) {
 #pragma unroll
     for (int k = 0; k < KA_HELD; ++k) {
@@ -81,6 +74,16 @@ __global__ void __launch_bounds__(KA_THREADS) kv_cache_append_kernel(const KaArg
       if (v < nv) held[k].load(src + at(v));
       else held[k].zero();
     }
+  }
+  if (id < 0 || id >= a.pages) bad = true;
+  if (bad && threadIdx.x == 0) atomicExch(&g_cache_append_status, 1);
+  if (id < 0 || id >= a.pages) return;
+  float *sp = a.scale[side] + id * a.H + h;
+  uint8_t *dst = a.pool[side] + (id * a.H + h) * (int64_t)a.T * a.D;
+  const float before = older ? *sp : 0.0f;
+  // ---- the largest magnitude of the new values ----
+  uint32_t m = 0u;
+  if constexpr (VEC) {
 #pragma unroll
     for (int k = 0; k < KA_HELD; ++k) m = max(m, mag8(held[k]));
     for (int v = threadIdx.x + KA_HELD * KA_THREADS; v < nv; v += KA_THREADS) {
