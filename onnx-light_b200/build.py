@@ -65,7 +65,7 @@ def _binding() -> None:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[f"-isystem{i}" for i in includes], src, "-o", BINDING,
            f"-L{os.path.join(root, 'lib')}", f"-L{os.path.join(cuda, 'lib64')}", "-ltorch_python",
-           "-ltorch_cpu", "-lc10", "-lc10_cuda", "-l:libcudart.so.12"]
+           "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-l:libcudart.so.12"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"building {BINDING} failed:\n{r.stdout}\n{r.stderr}")

@@ -13,8 +13,7 @@ struct SmArgs {
 };
 
 // Few rows (scaled_matmul_skinny.cu).
-constexpr int64_t kScaledSkinnyRows = 64;
-bool scaled_skinny_eligible(const SmArgs &g);
+bool scaled_skinny_eligible(const SmArgs &g, bool f8);
 int scaled_skinny_launch(const SmArgs &g, int y_dtype, bool f8, cudaStream_t st);
 
 // Tensor-core tiles (scaled_matmul_tc.cu).

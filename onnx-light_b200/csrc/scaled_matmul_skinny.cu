@@ -121,16 +121,19 @@ template <typename T, typename Q> int pick(const SmArgs &g, cudaStream_t st) {
   const int64_t tiles = (g.N + 15) / 16;
   if (g.M <= 8) scaled_mm_skinny<T, Q, 1, 1, 4><<<(unsigned)tiles, SK_WARPS * 32, 0, st>>>(g);
   else if (g.M <= 16) scaled_mm_skinny<T, Q, 2, 1, 4><<<(unsigned)tiles, SK_WARPS * 32, 0, st>>>(g);
-  else if (g.M <= 32) scaled_mm_skinny<T, Q, 4, 1, 2><<<(unsigned)tiles, SK_WARPS * 32, 0, st>>>(g);
-  else scaled_mm_skinny<T, Q, 8, 1, 2><<<(unsigned)tiles, SK_WARPS * 32, 0, st>>>(g);
+  else scaled_mm_skinny<T, Q, 4, 1, 2><<<(unsigned)tiles, SK_WARPS * 32, 0, st>>>(g);
   B2_LAUNCH_CHECK();
   return B2_OK;
 }
 
 } // namespace
 
-bool scaled_skinny_eligible(const SmArgs &g) {
-  return g.M <= kScaledSkinnyRows && g.K > 0 && g.K % 16 == 0 && aligned(g.a, 16) && aligned(g.w, 16) &&
+// Against the tcgen05 kernel (us, K x N, here / there): INT8 16 rows 4096 x 11008 14.8 / 17.6, 32 rows
+// 19.7 / 12.3; FLOAT8, whose mma.sync is slower, 8 rows 14.1 / 17.7, 16 rows 18.9 / 17.8; with a
+// weight of a million codes, where a launch counts, 32 rows 2.8 / 4.2, 64 rows 5.0 / 4.5.
+bool scaled_skinny_eligible(const SmArgs &g, bool f8) {
+  const int64_t rows = g.N * g.K <= (1 << 21) ? 32 : f8 ? 8 : 16;
+  return g.M <= rows && g.K > 0 && g.K % 16 == 0 && aligned(g.a, 16) && aligned(g.w, 16) &&
          g.N < ((int64_t)1 << 34);
 }
 

@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -130,7 +131,7 @@ bool device_of(PyObject *o, int *device) {
 }
 
 at::Tensor empty_like_shape(at::IntArrayRef shape, at::ScalarType type, int device) {
-  return at::empty(shape, at::TensorOptions().dtype(type).device(at::kCUDA, device));
+  return at::detail::empty_cuda(shape, type, at::Device(at::kCUDA, (c10::DeviceIndex)device), std::nullopt);
 }
 
 // One zeroed buffer per (device, stream), grown on demand: calls on one stream are ordered, and
