@@ -416,6 +416,10 @@ __global__ void __launch_bounds__(CP_THREADS, 1)
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const int qi = q0 + row % g.np, pos = sp.past + qi; // position of the row's query
     const bool counts = qi < sp.count;
+    // keys the row sees: first_key .. last_key, and the sinks
+    const int last_key = a.causal ? min(pos, sp.total - 1) : sp.total - 1;
+    const int first_key = win ? pos - a.window : 0;
+    auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }; // bits < n
     auto softmax_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(CP_SOFT * 32) : "memory"); };
     float qf = 1.0f; // power of two taken out of the row's queries
     {
@@ -497,22 +501,25 @@ __global__ void __launch_bounds__(CP_THREADS, 1)
           v[32 + e] = __uint_as_float(r1[e]);
         }
         if (!__all_sync(0xffffffffu, plain && !need_mask)) {
-          // every score in base-2 units, -inf where the row does not see the key; pages out of
-          // range (flag 0) hold no keys
+          // every score in base-2 units, -inf where the row does not see the key: one bit per key;
+          // pages out of range (flag 0) hold no keys
+          uint32_t bits[2];
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const int base = key0 + w * 32;
+            bits[w] = below(last_key + 1 - base) & (~below(first_key - base) | below(a.sinks - base));
+          }
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const float flag = sc[(j & 3) * 8 + half * 4 + c].w;
-            bool any = false;
+            const uint32_t flag = __float_as_uint(sc[(j & 3) * 8 + half * 4 + c].w);
+            const uint32_t seen = flag ? (bits[c >> 1] >> ((c & 1) * 16)) & 0xffffu : 0u;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const int key = key0 + c * 16 + e;
               float x = v[c * 16 + e] * vk[c];
               if (a.softcap > 0.0f) x = a.softcap * tanhf(x * kLn2 / a.softcap) * kLog2E;
-              const bool seen = flag != 0.0f && key < sp.total && ca_sees(a, pos, key);
-              any = any || seen;
-              v[c * 16 + e] = seen ? x : -INFINITY;
+              v[c * 16 + e] = seen >> e & 1u ? x : -INFINITY;
             }
-            poison = poison || (any && inv[c] != inv[c]); // it sees values that are not finite
+            poison = poison || (seen != 0u && inv[c] != inv[c]); // it sees values that are not finite
             if (inv[c] != inv[c]) inv[c] = 0.0f;
             vk[c] = 1.0f;
           }

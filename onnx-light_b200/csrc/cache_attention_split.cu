@@ -20,7 +20,7 @@
 // v_scale is held to [-60, 110] so that p cannot overflow; a scale below only makes its products
 // smaller.
 //
-// Data path: tiles of 32 tokens (K and V, [32][128 B] with the 128-byte swizzle) through a TMA ring
+// Data path: tiles of 32 tokens (K and V, 128 bytes a token, 128-byte swizzle) through a TMA ring
 // filled by one producer warp.  Page numbers and scales are fetched for the next 8 to 32 tiles at
 // once, one page chunk a lane; the first tiles' copies start before their scales arrive.  Each
 // tile is one consumer warp's: the swizzle makes the fragment reads (16 bytes a lane) free of
@@ -32,6 +32,7 @@
 // by its last arriver in CTA order, so results do not depend on timing.
 #include <algorithm>
 
+#include "attn_math.cuh"
 #include "cache_attention.cuh"
 #include "tc_common.cuh"
 
@@ -44,18 +45,18 @@ namespace {
 
 using namespace q8;
 
-constexpr int CS_KEYS = 32; // tokens per tile
+constexpr int KEYS = 32; // tokens per tile
 constexpr float CS_LIFT = 15.0f; // log2 of the largest p * v_scale
-constexpr uint32_t CS_BOX = CS_KEYS * 128; // one 128-byte-wide tile of codes
 constexpr size_t CS_SMEM_MAX = 232448;
 constexpr int CS_CTAS = 160; // at most, one per SM
 
 template <int DP, int NT> struct CsLayout {
+  static constexpr uint32_t BOX = KEYS * 128;             // a 128-byte-wide tile of codes
   static constexpr int NB = DP == 256 ? 2 : 1;            // 128-byte boxes per row
   // Consumer warps: 11 and the producer share the register file at 168 each, 7 at 255.
   static constexpr int WARPS = NT == 1 && DP <= 128 ? 11 : DP <= 128 || NT == 1 ? 7 : 4;
   static constexpr int THREADS = (WARPS + 1) * 32;
-  static constexpr uint32_t STAGE = 2 * NB * CS_BOX;      // K boxes, V boxes
+  static constexpr uint32_t STAGE = 2 * NB * BOX;      // K boxes, V boxes
   static constexpr int W = DP + 4;                        // a row's O, m, l (16-byte rows)
   static constexpr uint32_t MERGE = WARPS * 8 * NT * W * 4;
   static constexpr uint32_t FIXED = 1024 + MERGE + 4096;  // alignment, merge, barriers, scales
@@ -65,8 +66,8 @@ template <int DP, int NT> struct CsLayout {
                                     : 24;
   static constexpr uint32_t OFF_MERGE = STAGES * STAGE;
   static constexpr uint32_t OFF_BAR = OFF_MERGE + MERGE;  // full, empty
-  static constexpr uint32_t OFF_SC = OFF_BAR + 24 * 16;   // float4 [STAGES][4]
-  static constexpr uint32_t OFF_MISC = OFF_SC + 24 * 64;
+  static constexpr uint32_t OFF_SC = OFF_BAR + 24 * 16;   // float4 [STAGES][KEYS / 8]
+  static constexpr uint32_t OFF_MISC = OFF_SC + STAGES * KEYS * 2;
   static constexpr size_t SMEM = OFF_MISC + 256 + 1024;
   static_assert(STAGES >= WARPS && STAGES >= 4 && SMEM <= CS_SMEM_MAX, "shared memory");
 };
@@ -74,7 +75,7 @@ template <int DP, int NT> struct CsLayout {
 struct CsArgs {
   CaArgs c;
   int packs, rows;  // packs of 8 NT rows of a KV head's `rows` = S * group
-  int chunk;        // tokens per TMA box: a power of two, 8 to 32, that divides the page
+  int chunk, shift; // tokens per TMA box: a power of two (2^shift), 8 to KEYS, that divides the page
   int align_pairs;  // CTA ranges start at pair boundaries (more pairs than counters)
   float *partials;  // [grid][2][8 NT][DP + 4]: O, m, l
   uint32_t *counters;
@@ -129,11 +130,6 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
   return v;
 }
-// 16-byte unit u (0..7) of row r in a [rows][128 B] box written with the 128-byte swizzle.
-__device__ __forceinline__ uint32_t unit_at(uint32_t base, int r, int u) {
-  return base + (uint32_t)(r * 128 + ((u ^ (r & 7)) << 4));
-}
-
 // The tiles of sequence b: the window's (from the first query's) and the sinks' before it.
 struct CsSeq {
   CaSpan sp;
@@ -143,14 +139,14 @@ __device__ __forceinline__ CsSeq cs_seq(const CaArgs &a, int b, bool *bad) {
   CsSeq s;
   s.sp = ca_span(a, b, bad);
   const bool win = a.causal && a.window >= 0;
-  s.first = win ? max(0, s.sp.past - a.window) / CS_KEYS : 0;
-  s.sink_tiles = win ? min((min(a.sinks, s.sp.total) + CS_KEYS - 1) / CS_KEYS, s.first) : 0;
-  s.tiles = s.sp.count > 0 ? s.sink_tiles + (s.sp.total + CS_KEYS - 1) / CS_KEYS - s.first : 0;
+  s.first = win ? max(0, s.sp.past - a.window) / KEYS : 0;
+  s.sink_tiles = win ? min((min(a.sinks, s.sp.total) + KEYS - 1) / KEYS, s.first) : 0;
+  s.tiles = s.sp.count > 0 ? s.sink_tiles + (s.sp.total + KEYS - 1) / KEYS - s.first : 0;
   s.tiles = max(s.tiles, 1); // a sequence without new tokens still gets its zeros written
   return s;
 }
 __device__ __forceinline__ int cs_key0(const CsSeq &s, int tile) {
-  return (tile < s.sink_tiles ? tile : s.first + tile - s.sink_tiles) * CS_KEYS;
+  return (tile < s.sink_tiles ? tile : s.first + tile - s.sink_tiles) * KEYS;
 }
 
 // A walk over the units in order.
@@ -182,7 +178,7 @@ __device__ __forceinline__ bool cs_live(const CsArgs &g, const CsSeq &s, int fir
   if (last < first || key0 >= s.sp.total) return false;
   if (!g.c.causal) return true;
   if (key0 > last) return false;
-  return g.c.window < 0 || key0 + CS_KEYS > first - g.c.window || key0 < g.c.sinks;
+  return g.c.window < 0 || key0 + KEYS > first - g.c.window || key0 < g.c.sinks;
 }
 
 // Sum of v over the block and the sum over the threads before this one; every thread calls it.
@@ -219,6 +215,9 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
     cache_attn_split(const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v, const CsArgs g) {
   using L = CsLayout<DP, NT>;
+  constexpr uint32_t BOX = L::BOX;
+  constexpr int CHUNKS = KEYS / 8; // at most, per tile
+  constexpr int MT = KEYS / 16;    // 16-token tiles
   constexpr int STAGES = L::STAGES, WARPS = L::WARPS, NB = L::NB, RP = 8 * NT;
   constexpr int KS = DP / 16;                 // k16 steps of Q.K; M tiles of P.V
   extern __shared__ uint8_t dsm[];
@@ -336,7 +335,7 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
     // read two batches ahead and scales one, so no batch waits for them; within a batch, groups of
     // up to 8 tiles go through the ring's protocol together, one tile a lane
     // (at most half the ring, so that a group's stages are distinct and the others stay in flight).
-    const int nch = CS_KEYS / g.chunk, per = 32 / nch, grp = min(per, min(8, STAGES / 2));
+    const int nch = KEYS >> g.shift, per = 32 / nch, grp = min(per, min(8, STAGES / 2));
     const int my = lane / nch, ch = lane % nch;
     const uint32_t chunk_bytes = (uint32_t)(g.chunk * 128 * 2 * NB);
     if (lane == 0) {
@@ -384,8 +383,8 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
         uint8_t *st = sm + s * L::STAGE + ch * g.chunk * 128;
 #pragma unroll
         for (int x = 0; x < NB; ++x) {
-          tc::tma_load_3d(st + x * CS_BOX, &map_k, &full[s], x * 128, c0.row, z0);
-          tc::tma_load_3d(st + (NB + x) * CS_BOX, &map_v, &full[s], x * 128, c0.row, z0);
+          tc::tma_load_3d(st + x * BOX, &map_k, &full[s], x * 128, c0.row, z0);
+          tc::tma_load_3d(st + (NB + x) * BOX, &map_v, &full[s], x * 128, c0.row, z0);
         }
       };
       // The first fill of the ring: every copy starts before its scales are waited for (a copy may
@@ -415,7 +414,7 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
           break;
         }
         if (act) // key scale in score units; value scale; its logarithm; validity
-          sc[s * 4 + ch] = make_float4(ks * a.scale * kLog2E, vs, fminf(fmaxf(log2f(vs), -60.0f), 110.0f),
+          sc[s * CHUNKS + ch] = make_float4(ks * a.scale * kLog2E, vs, fminf(fmaxf(log2f(vs), -60.0f), 110.0f),
                                        z0 >= 0 ? 1.0f : 0.0f);
         __syncwarp();
         if (act && ch == 0)
@@ -440,6 +439,9 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
   const int gq = lane >> 2, t = lane & 3;
   bool ok = true;
   int first_pair = -1; // number of the range's first pair
+  const uint32_t smem0 = tc::smem_u32(sm);
+  const uint32_t k_at = gq * 128 + (((DP == 64 ? t : 2 * t) ^ gq) << 4);
+  const uint32_t v_at = 2 * t * 128 + ((DP == 64 ? (gq >> 1) ^ (2 * t) : gq ^ (2 * t)) << 4) + (DP == 64 ? (gq & 1) * 8 : 0);
   int seg0 = 0;
   while (seg0 < nun) {
     cs_seek(g, walk, u0 + seg0);
@@ -531,105 +533,127 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
       ok = __all_sync(0xffffffffu, ok);
       const int key0 = cs_key0(seq, walk.tile + (i - seg0));
       if (ok && cs_live(g, seq, pos_first, pos_last, key0)) {
-        const uint32_t kb = tc::smem_u32(sm + s * L::STAGE), vb = kb + NB * CS_BOX;
-        // scales of the tokens of this lane's S rows: gq and gq + 8 of each 16
-        float4 c4[2][2];
-        bool all = true;
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            c4[mt][h] = sc[s * 4 + (mt * 16 + h * 8 + gq) / g.chunk];
-            all = all && c4[mt][h].w != 0.0f;
-          }
-        all = __all_sync(0xffffffffu, all);
-        const bool whole = all && key0 + CS_KEYS <= seq.sp.total;
+        // The 16-byte unit u of row r of a box lies at r * 128 + ((u ^ (r & 7)) << 4).  A lane's K rows
+        // are gq (mod 8), its V rows 2t and 2t + 1, so the exclusive or leaves two places for each.
+        const uint32_t kb = smem0 + s * L::STAGE, vb = kb + NB * BOX;
+        const uint32_t ka = kb + k_at, va[2] = {vb + v_at, vb + (v_at ^ 16) + 128};
+        // scales of the tokens of this lane's S rows (gq and gq + 8 of each 16)
+        auto scales = [&](int mt, int h) { return sc[s * CHUNKS + ((mt * 16 + h * 8 + gq) >> g.shift)]; };
+        const bool all = __all_sync(0xffffffffu, lane >= KEYS >> g.shift || sc[s * CHUNKS + lane].w != 0.0f);
+        const bool whole = all && key0 + KEYS <= seq.sp.total;
         if (!whole) {
           // rows that hold no token of this sequence: their V codes must not reach the MMA
 #pragma unroll 1
-          for (int r = lane >> 3; r < CS_KEYS; r += 4) {
-            if (key0 + r >= seq.sp.total || sc[s * 4 + r / g.chunk].w == 0.0f)
+          for (int r = lane >> 3; r < KEYS; r += 4) {
+            if (key0 + r >= seq.sp.total || sc[s * CHUNKS + (r >> g.shift)].w == 0.0f)
 #pragma unroll
               for (int x = 0; x < NB; ++x)
-                *reinterpret_cast<uint4 *>(sm + s * L::STAGE + (NB + x) * CS_BOX + r * 128 + (lane & 7) * 16) =
+                *reinterpret_cast<uint4 *>(sm + s * L::STAGE + (NB + x) * BOX + r * 128 + (lane & 7) * 16) =
                     make_uint4(0u, 0u, 0u, 0u);
           }
           tc::fence_proxy_async(); // before the stage's next TMA fill
           __syncwarp();
         }
         const bool need_mask =
-            !whole || (a.causal && (key0 + CS_KEYS - 1 > pos_first ||
-                                    (a.window >= 0 && key0 < pos_last - a.window && key0 + CS_KEYS > a.sinks))) ||
+            !whole || (a.causal && (key0 + KEYS - 1 > pos_first ||
+                                    (a.window >= 0 && key0 < pos_last - a.window && key0 + KEYS > a.sinks))) ||
             pos_last - seq.sp.past != (pack * RP + rows - 1) / a.group; // rows that do not count
         // ---- S^T = K . Q^T ----
         // With one tile of rows, even and odd steps have sums of their own: four short chains of MMAs.
         constexpr int CH = NT == 1 ? 2 : 1;
-        float sv[2][NT][4], sx[CH][2][NT][4];
+        float sv[MT][NT][4];
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
+        for (int m2 = 0; m2 < MT; m2 += 2) {
+          float sx[CH][2][NT][4];
+#pragma unroll
+          for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sx[c][mt][nt][e] = 0.0f;
+#pragma unroll
+          for (int x = 0; x < NB; ++x)
+#pragma unroll
+            for (int h = 0; h < (DP == 64 ? 1 : 2); ++h) {
+              uint32_t w[2][2][4];
+#pragma unroll
+              for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                  const uint4 v = lds128((h ? ka ^ 16 : ka) + x * BOX + (m2 + mt) * 2048 + r * 1024);
+                  w[mt][r][0] = v.x;
+                  w[mt][r][1] = v.y;
+                  w[mt][r][2] = v.z;
+                  w[mt][r][3] = v.w;
+                }
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt) {
+                  uint32_t a0, a1, a2, a3;
+                  to_half<Q>(w[mt][0][q], a0, a2);
+                  to_half<Q>(w[mt][1][q], a1, a3);
+                  const int k = x * 8 + h * 4 + q;
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt)
+                    mma16816(sx[q % CH][mt][nt], a0, a1, a2, a3, qb[nt][k][0], qb[nt][k][1]);
+                }
+            }
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) sx[c][mt][nt][e] = 0.0f;
-#pragma unroll
-        for (int x = 0; x < NB; ++x)
-#pragma unroll
-          for (int h = 0; h < (DP == 64 ? 1 : 2); ++h) {
-            const int u = DP == 64 ? t : 2 * t + h;
-            uint32_t w[2][2][4];
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                const uint4 v = lds128(unit_at(kb + x * CS_BOX, mt * 16 + r * 8 + gq, u));
-                w[mt][r][0] = v.x;
-                w[mt][r][1] = v.y;
-                w[mt][r][2] = v.z;
-                w[mt][r][3] = v.w;
-              }
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-              for (int mt = 0; mt < 2; ++mt) {
-                uint32_t a0, a1, a2, a3;
-                to_half<Q>(w[mt][0][q], a0, a2);
-                to_half<Q>(w[mt][1][q], a1, a3);
-                const int k = x * 8 + h * 4 + q;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                  mma16816(sx[q % CH][mt][nt], a0, a1, a2, a3, qb[nt][k][0], qb[nt][k][1]);
-              }
-          }
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              sv[mt][nt][e] = CH == 2 ? sx[0][mt][nt][e] + sx[CH - 1][mt][nt][e] : sx[0][mt][nt][e];
+              for (int e = 0; e < 4; ++e)
+                sv[m2 + mt][nt][e] = CH == 2 ? sx[0][mt][nt][e] + sx[CH - 1][mt][nt][e] : sx[0][mt][nt][e];
+        }
         // ---- scores in base 2, masks, the running reference ----
-        float mx[NT][2];
+        float mx[NT][2], lz[MT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 c = scales(mt, h);
+            lz[mt][h] = c.z;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                sv[mt][nt][2 * h + e] *= std::is_same<T, __half>::value ? c.x : c.x * qf[nt][e];
+          }
+        if (a.softcap > 0.0f) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                sv[mt][nt][e] = a.softcap * tanhf(sv[mt][nt][e] * kLn2 / a.softcap) * kLog2E;
+        }
+        if (need_mask) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int j = key0 + mt * 16 + h * 8 + gq;
+              const bool has = scales(mt, h).w != 0.0f;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (!(has && j <= hi[nt][e] && (j >= lo[nt][e] || j < a.sinks))) sv[mt][nt][2 * h + e] = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float4 c = c4[mt][e >> 1];
-              float v = sv[mt][nt][e] * qf[nt][e & 1] * c.x;
-              if (a.softcap > 0.0f) v = a.softcap * tanhf(v * kLn2 / a.softcap) * kLog2E;
-              if (need_mask) {
-                const int j = key0 + mt * 16 + (e >> 1) * 8 + gq;
-                const bool seen = j <= hi[nt][e & 1] && (j >= lo[nt][e & 1] || j < a.sinks) && c.w != 0.0f;
-                if (!seen) v = -INFINITY;
-              }
-              sv[mt][nt][e] = v;
-              mx[nt][e & 1] = fmaxf(mx[nt][e & 1], v + c.z);
-            }
+            for (int e = 0; e < 4; ++e) mx[nt][e & 1] = fmaxf(mx[nt][e & 1], sv[mt][nt][e] + lz[mt][e >> 1]);
         float corr[NT][2], ref[NT][2];
         bool moved = false;
 #pragma unroll
@@ -640,7 +664,7 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
             for (int w = 4; w < 32; w <<= 1) mx[nt][e] = fmaxf(mx[nt][e], __shfl_xor_sync(0xffffffffu, mx[nt][e], w));
             const float mn = fmaxf(m_run[nt][e], mx[nt][e]);
             const float base = mn == -INFINITY ? 0.0f : mn;
-            corr[nt][e] = exp2f(m_run[nt][e] - base);
+            corr[nt][e] = ex2(m_run[nt][e] - base);
             ref[nt][e] = base - CS_LIFT;
             moved = moved || mn != m_run[nt][e];
             m_run[nt][e] = mn;
@@ -657,39 +681,42 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
           }
         }
         // ---- P^T fragments ----
-        uint32_t pb[2][NT][2];
+        uint32_t pb[MT][NT][2];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float p[4];
+          for (int h = 0; h < 2; ++h) {
+            const float vs = scales(mt, h).y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float v = sv[mt][nt][e];
-              p[e] = exp2f(v - ref[nt][e & 1]);
-              l_run[nt][e & 1] += p[e];
-              // a key that is not seen has p = 0 whatever its page's scale is
-              p[e] = v == -INFINITY ? 0.0f : p[e] * c4[mt][e >> 1].y;
+            for (int nt = 0; nt < NT; ++nt) {
+              float p[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float v = sv[mt][nt][2 * h + e];
+                p[e] = ex2(v - ref[nt][e]);
+                l_run[nt][e] += p[e];
+                p[e] *= vs;
+                // a key that is not seen has p = 0 whatever its page's scale is
+                if (need_mask && v == -INFINITY) p[e] = 0.0f;
+              }
+              pb[mt][nt][h] = transpose8(half2_of(p[0], p[1]));
             }
-            pb[mt][nt][0] = transpose8(half2_of(p[0], p[1]));
-            pb[mt][nt][1] = transpose8(half2_of(p[2], p[3]));
           }
         // ---- O^T += V^T . P^T ----
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const int r = mt * 16 + 2 * t;
+        for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
           for (int x = 0; x < NB; ++x) {
             uint32_t w[4][4]; // [token 2t, 2t + 1, 2t + 8, 2t + 9][4 columns each]
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const int rr = r + (q & 1) + (q >> 1) * 8;
+              const uint32_t at = va[q & 1] + mt * 2048 + (q >> 1) * 1024;
               if constexpr (DP == 64) {
-                const uint2 v = lds64(unit_at(vb, rr, gq >> 1) + (gq & 1) * 8);
+                const uint2 v = lds64(at);
                 w[q][0] = v.x;
                 w[q][1] = v.y;
               } else {
-                const uint4 v = lds128(unit_at(vb + x * CS_BOX, rr, gq));
+                const uint4 v = lds128(at + x * BOX);
                 w[q][0] = v.x;
                 w[q][1] = v.y;
                 w[q][2] = v.z;
@@ -923,7 +950,7 @@ int dp_of(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 bool cache_attn_split_eligible(const CaArgs &a) {
   const int64_t rows = (int64_t)a.S * a.group, nt = cs_nt(rows, dp_of(a.D));
   const int64_t packs = (rows + 8 * nt - 1) / (8 * nt);
-  const int64_t tiles = (int64_t)a.max_pages * a.T / CS_KEYS + 2;
+  const int64_t tiles = (int64_t)a.max_pages * a.T / KEYS + 2;
   return a.D % 16 == 0 && a.D <= 256 && a.T % 8 == 0 && aligned(a.q, 16) && aligned(a.k, 16) &&
          aligned(a.v, 16) && aligned(a.y, 8) && a.pages > 0 && rows < ((int64_t)1 << 30) &&
          (double)a.B * a.Hkv * packs * tiles < 1e9;
@@ -940,7 +967,9 @@ int cache_attn_split_launch(const CaArgs &a, bool f16, bool f8, void *ws, cudaSt
   g.c = a;
   g.rows = a.S * a.group;
   g.packs = (g.rows + 8 * nt - 1) / (8 * nt);
-  g.chunk = a.T % 32 == 0 ? 32 : a.T % 16 == 0 ? 16 : 8;
+  g.shift = 3;
+  while ((1 << g.shift) < KEYS && a.T % (2 << g.shift) == 0) ++g.shift;
+  g.chunk = 1 << g.shift;
   g.align_pairs = (int64_t)a.B * a.Hkv * g.packs > (int64_t)kMaxCounters;
   g.counters = static_cast<uint32_t *>(ws);
   g.partials = reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + kCounterBytes);
