@@ -53,9 +53,9 @@ constexpr int CS_CTAS = 160; // at most, one per SM
 template <int DP, int NT> struct CsLayout {
   static constexpr uint32_t BOX = KEYS * 128;             // a 128-byte-wide tile of codes
   static constexpr int NB = DP == 256 ? 2 : 1;            // 128-byte boxes per row
-  // Consumer warps: 11 and the producer share the register file at 168 each, 7 at 255.
-  static constexpr int WARPS = NT == 1 && DP <= 128 ? 11 : DP <= 128 || NT == 1 ? 7 : 4;
-  static constexpr int THREADS = (WARPS + 1) * 32;
+  // Consumer warps: 10 and the two producers share the register file at 168 each, 6 at 255.
+  static constexpr int WARPS = NT == 1 && DP <= 128 ? 10 : DP <= 128 || NT == 1 ? 6 : 4;
+  static constexpr int THREADS = (WARPS + 2) * 32;
   static constexpr uint32_t STAGE = 2 * NB * BOX;      // K boxes, V boxes
   static constexpr int W = DP + 4;                        // a row's O, m, l (16-byte rows)
   static constexpr uint32_t MERGE = WARPS * 8 * NT * W * 4;
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&full[i], 2);  // both producers
       tc::mbar_init(&empty[i], 1); // one consumer warp per stage
     }
     flags[0] = 0;
@@ -329,19 +329,20 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
   }
   const int nun = u1 - u0;
 
-  if (warp == WARPS) {
-    // ------------------------------ producer ------------------------------
+  if (warp >= WARPS) {
+    // ------------------------------ producers ------------------------------
+    // One warp brings the keys and the scales, the other the values (a lane's copies are issued one
+    // after the other, at about 170 cycles each: with one warp for both they set the pace).
     // Lane (my, ch) brings chunk ch of tile my of each batch of `per` tiles.  Page numbers are
     // read two batches ahead and scales one, so no batch waits for them; within a batch, groups of
     // up to 8 tiles go through the ring's protocol together, one tile a lane
     // (at most half the ring, so that a group's stages are distinct and the others stay in flight).
     const int nch = KEYS >> g.shift, per = 32 / nch, grp = min(per, min(8, STAGES / 2));
     const int my = lane / nch, ch = lane % nch;
-    const uint32_t chunk_bytes = (uint32_t)(g.chunk * 128 * 2 * NB);
-    if (lane == 0) {
-      tc::prefetch_tensormap(&map_k);
-      tc::prefetch_tensormap(&map_v);
-    }
+    const bool values = warp > WARPS;
+    const uint32_t chunk_bytes = (uint32_t)(g.chunk * 128 * NB);
+    const CUtensorMap *map = values ? &map_v : &map_k;
+    if (lane == 0) tc::prefetch_tensormap(map);
     struct Chunk {
       int id, row, kvh; // page, row in the page
       bool live;        // a key of it may be seen
@@ -375,17 +376,14 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
     int issued = 0;
     Chunk c0 = find(my), c1 = find(per + my);
     int z0 = place(c0);
-    float ks = z0 >= 0 ? a.ks[z0] : 0.0f, vs = z0 >= 0 ? a.vs[z0] : 0.0f;
+    float ks = !values && z0 >= 0 ? a.ks[z0] : 0.0f, vs = !values && z0 >= 0 ? a.vs[z0] : 0.0f;
     for (int i0 = 0; i0 < nun && !stop; i0 += per) {
       const int i = i0 + my, s = i % STAGES;
       const uint32_t have = __ballot_sync(0xffffffffu, z0 >= 0);
       auto copy = [&] { // this lane's boxes
-        uint8_t *st = sm + s * L::STAGE + ch * g.chunk * 128;
+        uint8_t *st = sm + s * L::STAGE + (values ? NB * BOX : 0) + ch * g.chunk * 128;
 #pragma unroll
-        for (int x = 0; x < NB; ++x) {
-          tc::tma_load_3d(st + x * BOX, &map_k, &full[s], x * 128, c0.row, z0);
-          tc::tma_load_3d(st + (NB + x) * BOX, &map_v, &full[s], x * 128, c0.row, z0);
-        }
+        for (int x = 0; x < NB; ++x) tc::tma_load_3d(st + x * BOX, map, &full[s], x * 128, c0.row, z0);
       };
       // The first fill of the ring: every copy starts before its scales are waited for (a copy may
       // land before its bytes are expected; the phase stays open until the arrival below).
@@ -393,7 +391,7 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
       if (early && z0 >= 0) copy();
       // the next batch's scales, and the pages of the one after
       const int z1 = place(c1);
-      const float ks1 = z1 >= 0 ? a.ks[z1] : 0.0f, vs1 = z1 >= 0 ? a.vs[z1] : 0.0f;
+      const float ks1 = !values && z1 >= 0 ? a.ks[z1] : 0.0f, vs1 = !values && z1 >= 0 ? a.vs[z1] : 0.0f;
       const Chunk c2 = find(i + 2 * per);
       for (int k = 0; k < per && i0 + k < nun; k += grp) {
         const bool act = my >= k && my < k + grp && i < nun;
@@ -413,7 +411,7 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
           stop = true;
           break;
         }
-        if (act) // key scale in score units; value scale; its logarithm; validity
+        if (act && !values) // key scale in score units; value scale; its logarithm; validity
           sc[s * CHUNKS + ch] = make_float4(ks * a.scale * kLog2E, vs, fminf(fmaxf(log2f(vs), -60.0f), 110.0f),
                                        z0 >= 0 ? 1.0f : 0.0f);
         __syncwarp();
