@@ -14,11 +14,11 @@
 // lose low bits); and p * v_scale, relative to the largest such product of the row, so 2^-11 of
 // what it contributes.  The denominator sums the unrounded p.
 //
-// The running reference of a row is m = max_j (s_j + log2 v_scale_j): with p_j = 2^(s_j - m + 15) in
+// The running reference of a row is m ~ max_j (s_j + log2 v_scale_j): with p_j = 2^(s_j - m + 7) in
 // fp32, p_j v_scale_j is at most 2^15 for every token, however far the pages' scales lie apart, and
-// keeps its 11 bits down to 2^-29 of the largest (FLOAT16's normal range ends at 2^-14).  log2
-// v_scale is held to [-60, 110] so that p cannot overflow; a scale below only makes its products
-// smaller.
+// keeps its 11 bits down to 2^-21 of the largest and below (FLOAT16's normal range ends at 2^-14).
+// log2 v_scale is held to [-60, 110] so that p cannot overflow; a scale below only makes its
+// products smaller.
 //
 // Data path: tiles of 32 tokens (K and V, 128 bytes a token, 128-byte swizzle) through a TMA ring
 // filled by one producer warp.  Page numbers and scales are fetched for the next 8 to 32 tiles at
@@ -46,7 +46,7 @@ namespace {
 using namespace q8;
 
 constexpr int KEYS = 32; // tokens per tile
-constexpr float CS_LIFT = 15.0f; // log2 of the largest p * v_scale
+constexpr float CS_TOP = 15.0f, CS_BASE = 7.0f; // log2 of the largest p * v_scale, and after a move of m
 constexpr size_t CS_SMEM_MAX = 232448;
 constexpr int CS_CTAS = 160; // at most, one per SM
 
@@ -522,7 +522,6 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
     // a parity wait cannot be satisfied by the fill before last.
     for (int i = seg0 + ((warp - seg0 % WARPS + WARPS) % WARPS); i < seg1; i += WARPS) {
       const int s = i % STAGES;
-      if (ok && flags[0]) ok = false;
       if (ok && !tc::mbar_wait(&full[s], (i / STAGES) & 1)) {
         atomicExch(&g_cache_attn_split_status, tc::kTimeoutFull);
         flags[0] = 1;
@@ -652,32 +651,36 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) mx[nt][e & 1] = fmaxf(mx[nt][e & 1], sv[mt][nt][e] + lz[mt][e >> 1]);
-        float corr[NT][2], ref[NT][2];
-        bool moved = false;
+        // m moves only when a product would pass 2^15 (then to 2^7), so most tiles cost one vote instead
+        // of a maximum over the lanes and a pass over the sums
+        bool over = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
+          for (int e = 0; e < 2; ++e) over = over || mx[nt][e] > m_run[nt][e] + (CS_TOP - CS_BASE);
+        if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-            for (int w = 4; w < 32; w <<= 1) mx[nt][e] = fmaxf(mx[nt][e], __shfl_xor_sync(0xffffffffu, mx[nt][e], w));
-            const float mn = fmaxf(m_run[nt][e], mx[nt][e]);
-            const float base = mn == -INFINITY ? 0.0f : mn;
-            corr[nt][e] = ex2(m_run[nt][e] - base);
-            ref[nt][e] = base - CS_LIFT;
-            moved = moved || mn != m_run[nt][e];
-            m_run[nt][e] = mn;
-          }
-        if (__any_sync(0xffffffffu, moved)) {
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            l_run[nt][0] *= corr[nt][0];
-            l_run[nt][1] *= corr[nt][1];
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
-            for (int k = 0; k < KS; ++k)
+              for (int w = 4; w < 32; w <<= 1) mx[nt][e] = fmaxf(mx[nt][e], __shfl_xor_sync(0xffffffffu, mx[nt][e], w));
+              const float mn = fmaxf(m_run[nt][e], mx[nt][e]);
+              const float corr = ex2(m_run[nt][e] - (mn == -INFINITY ? 0.0f : mn));
+              m_run[nt][e] = mn;
+              l_run[nt][e] *= corr;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[nt][k][e] *= corr[nt][e & 1];
-          }
+              for (int k = 0; k < KS; ++k) {
+                o[nt][k][e] *= corr;
+                o[nt][k][2 + e] *= corr;
+              }
+            }
         }
+        float ref[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) ref[nt][e] = (m_run[nt][e] == -INFINITY ? 0.0f : m_run[nt][e]) - CS_BASE;
         // ---- P^T fragments ----
         uint32_t pb[MT][NT][2];
 #pragma unroll
