@@ -186,14 +186,15 @@ extern "C" int b2_cache_attention(const b2_tensor *q, const b2_quantized_cache *
   const bool empty = B == 0 || S == 0;
   const bool prefill = !empty && (int64_t)a.S * a.group > 32 && cache_attn_prefill_eligible(a);
   const bool split = !empty && !prefill && cache_attn_split_eligible(a);
-  const int wr = workspace_check(workspace, workspace_bytes, split ? cache_attn_split_workspace(a) : 0);
+  const int wr = workspace_check(workspace, workspace_bytes,
+                                 split ? cache_attn_split_workspace(a) : prefill ? cache_attn_prefill_workspace(a) : 0);
   if (wr != 0) return wr > 0 ? B2_OK : wr;
   if (empty) return B2_OK;
   B2_ENFORCE(q->data && y->data, "%s: a tensor has no data.", op);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool f8 = cache->k->dtype == kF8E4M3FN;
-  if (prefill) return cache_attn_prefill_launch(a, q->dtype == kFloat16, f8, st);
-  B2_ENFORCE(!split || q8::aligned(workspace, 16), "%s: the workspace must be 16-byte aligned.", op);
+  B2_ENFORCE(q8::aligned(workspace, 16), "%s: the workspace must be 16-byte aligned.", op);
+  if (prefill) return cache_attn_prefill_launch(a, q->dtype == kFloat16, f8, workspace, st);
   if (split) return cache_attn_split_launch(a, q->dtype == kFloat16, f8, workspace, st);
   const unsigned grid = (unsigned)((B * Hq * S + CAA_WARPS - 1) / CAA_WARPS);
   if (q->dtype == kFloat16) {

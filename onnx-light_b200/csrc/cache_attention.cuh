@@ -48,7 +48,7 @@ int cache_attn_split_launch(const CaArgs &a, bool f16, bool f8, void *ws, cudaSt
 
 // Prompts on tcgen05 (cache_attention_prefill.cu).
 bool cache_attn_prefill_eligible(const CaArgs &a);
-int64_t cache_attn_prefill_ctas(const CaArgs &a);
-int cache_attn_prefill_launch(const CaArgs &a, bool f16, bool f8, cudaStream_t st);
+size_t cache_attn_prefill_workspace(const CaArgs &a);
+int cache_attn_prefill_launch(const CaArgs &a, bool f16, bool f8, void *ws, cudaStream_t st);
 
 } // namespace b2

@@ -22,6 +22,7 @@
 // Every mbarrier is waited phase by phase by the threads that depend on it, and no barrier can run
 // two phases ahead of a waiter.  All waits are bounded; after a time-out the CTA records a code,
 // waits for its MMAs in flight, frees its TMEM and returns.
+#include <algorithm>
 #include <type_traits>
 
 #include "attn_math.cuh"
@@ -66,6 +67,8 @@ template <int DP> struct CpLayout {
 struct CpArgs {
   CaArgs c;
   int qtiles, pk, np, hpacks;
+  int splits;         // CTAs that share a query tile's keys, at most
+  float *partials;    // [query tile][splits][128][DP + 4]: O, m, l
   float scale_log2;
   FastDiv div_t; // by the page size
   int chunk;     // keys per TMA box: a power of two, 16 to 128, that divides the page
@@ -94,6 +97,32 @@ template <typename Q> __device__ __forceinline__ void widen4(uint32_t w, uint32_
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// What a query tile's CTAs have to do.
+struct CpTile {
+  int b, h0, q0;                 // sequence, first query head, first query
+  CaSpan sp;
+  int first, sink_tiles, tiles;  // key tiles: the window's first, the sinks' before it, all
+  int parts;                     // CTAs that share them
+};
+__device__ __forceinline__ CpTile cp_tile(const CpArgs &g, int qtile, bool *bad) {
+  const CaArgs &a = g.c;
+  CpTile t{};
+  const int bhp = qtile / g.qtiles;
+  t.b = bhp / g.hpacks;
+  t.h0 = (bhp % g.hpacks) * g.pk;
+  t.q0 = (g.qtiles - 1 - qtile % g.qtiles) * g.np; // long rows first
+  t.sp = ca_span(a, t.b, bad);
+  if (t.q0 >= t.sp.count) return t; // no query of this tile counts
+  const int p_first = t.sp.past + t.q0, p_last = t.sp.past + min(t.q0 + g.np, t.sp.count) - 1;
+  const int kend = a.causal ? min(t.sp.total, p_last + 1) : t.sp.total;
+  const bool win = a.causal && a.window >= 0;
+  t.first = win ? max(0, p_first - a.window) / CP_N : 0;
+  t.sink_tiles = win ? min((min(a.sinks, kend) + CP_N - 1) / CP_N, t.first) : 0;
+  t.tiles = t.sink_tiles + (kend + CP_N - 1) / CP_N - t.first;
+  t.parts = min(g.splits, t.tiles);
+  return t;
 }
 
 template <typename T, typename Q, int DP>
@@ -127,15 +156,15 @@ __global__ void __launch_bounds__(CP_THREADS, 1)
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int qt = g.qtiles - 1 - (int)(blockIdx.x % g.qtiles); // long rows first
-  const int bhp = (int)(blockIdx.x / g.qtiles);
-  const int b = bhp / g.hpacks, h0 = (bhp % g.hpacks) * g.pk, kvh = h0 / a.group;
-  const int q0 = qt * g.np;
+  const int part = (int)(blockIdx.x % g.splits), qtile = (int)(blockIdx.x / g.splits);
   bool bad;
-  const CaSpan sp = ca_span(a, b, &bad);
+  const CpTile tile = cp_tile(g, qtile, &bad);
+  const int b = tile.b, h0 = tile.h0, kvh = h0 / a.group, q0 = tile.q0;
+  const CaSpan sp = tile.sp;
   if (bad && threadIdx.x == 0) atomicExch(&g_cache_attn_prefill_range, 1);
   T *yb = static_cast<T *>(a.y) + (int64_t)b * a.q_b;
   if (q0 >= sp.count) { // no query of this tile counts
+    if (part) return;
     const int cols = a.D / 8;
     for (int e = threadIdx.x; e < CP_M * cols; e += CP_THREADS) {
       const int row = e / cols, i = q0 + row % g.np;
@@ -145,14 +174,14 @@ __global__ void __launch_bounds__(CP_THREADS, 1)
     }
     return;
   }
-  // positions of the first and last query that counts; the tiles some of them see
+  // positions of the first and last query that counts; this CTA's share of the key tiles
   const int p_first = sp.past + q0, p_last = sp.past + min(q0 + g.np, sp.count) - 1;
-  const int kend = a.causal ? min(sp.total, p_last + 1) : sp.total;
   const bool win = a.causal && a.window >= 0;
-  const int first = win ? max(0, p_first - a.window) / CP_N : 0;
-  const int sink_tiles = win ? min((min(a.sinks, kend) + CP_N - 1) / CP_N, first) : 0;
-  const int ntiles = sink_tiles + (kend + CP_N - 1) / CP_N - first;
-  auto key0_of = [&](int j) { return (j < sink_tiles ? j : first + j - sink_tiles) * CP_N; };
+  const int first = tile.first, sink_tiles = tile.sink_tiles, parts = tile.parts;
+  if (part >= parts) return;
+  const int t0 = (int)((int64_t)part * tile.tiles / parts);
+  const int ntiles = (int)((int64_t)(part + 1) * tile.tiles / parts) - t0;
+  auto key0_of = [&](int j) { return (t0 + j < sink_tiles ? t0 + j : first + t0 + j - sink_tiles) * CP_N; };
 
   if (threadIdx.x == 0) {
     tc::mbar_init(q_full, CP_SOFT);
@@ -603,23 +632,34 @@ __global__ void __launch_bounds__(CP_THREADS, 1)
       tc::tc_fence_after();
       const float scale = l_sum == 0.0f ? 0.0f : 1.0f / l_sum; // a NaN stays
       T *yr = yb + (int64_t)(h0 + row / g.np) * a.q_h + (int64_t)qi * a.q_s;
-      uint32_t r[32];
+      float *mine = g.partials + (((size_t)qtile * g.splits + part) * CP_M + row) * (DP + 4);
+      if (parts > 1 && half == 0) *reinterpret_cast<float2 *>(mine + DP) = make_float2(m_ref, l_sum);
 #pragma unroll 1
       for (int c = 0; c < OC / 32; ++c) {
+        uint32_t r[32];
         tc::tmem_ld32(tmem + lane_off + CP_COL_O + half * OC + c * 32, r);
         tc::tmem_ld_wait();
-        if (qi < a.S) {
+        const int d0 = half * OC + c * 32;
+        if (parts > 1) { // several CTAs share the tile: cache_attn_prefill_join adds their O, m, l
+          if (counts) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              *reinterpret_cast<float4 *>(mine + d0 + q * 4) =
+                  make_float4(__uint_as_float(r[q * 4]), __uint_as_float(r[q * 4 + 1]), __uint_as_float(r[q * 4 + 2]),
+                              __uint_as_float(r[q * 4 + 3]));
+          }
+        } else if (qi < a.S) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const int d = half * OC + c * 32 + q * 8;
             float f[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = counts ? __uint_as_float(r[q * 8 + e]) * scale : 0.0f;
-            if (d < a.D) Raw8<T>::store(yr + d, f);
+            if (d0 + q * 8 < a.D) Raw8<T>::store(yr + d0 + q * 8, f);
           }
         }
       }
-    } else {
+    }
+    if (!fin) {
       atomicExch(&g_cache_attn_prefill_status, tc::kTimeoutFull);
       *abort_flag = 1;
     }
@@ -629,25 +669,82 @@ __global__ void __launch_bounds__(CP_THREADS, 1)
   if (warp == CP_MMA) tc::tmem_dealloc(tmem, CP_TMEM_COLS);
 }
 
+// Adds the parts of query tiles whose keys several CTAs shared, in order: one warp per query row, a
+// lane for four columns at a time.
+template <typename T, int DP> __global__ void __launch_bounds__(256) cache_attn_prefill_join(const CpArgs g) {
+  const int row = (int)(blockIdx.x % (CP_M / 8)) * 8 + (threadIdx.x >> 5), qtile = (int)(blockIdx.x / (CP_M / 8));
+  const int d = (threadIdx.x & 31) * 4;
+  bool bad;
+  const CpTile t = cp_tile(g, qtile, &bad);
+  const int qi = t.q0 + row % g.np;
+  if (t.parts <= 1 || qi >= g.c.S || d >= g.c.D) return;
+  T *y = static_cast<T *>(g.c.y) + (int64_t)t.b * g.c.q_b + (int64_t)(t.h0 + row / g.np) * g.c.q_h +
+         (int64_t)qi * g.c.q_s + d;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (qi < t.sp.count) {
+    constexpr int W = DP + 4;
+    const float *p = g.partials + ((size_t)qtile * g.splits * CP_M + row) * W;
+    float M = -INFINITY, l = 0.0f;
+    for (int c = 0; c < t.parts; c += 8) {
+      float2 ml[8];
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.0f);
+        v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (c + k < t.parts) {
+          const float *src = p + (size_t)(c + k) * CP_M * W;
+          ml[k] = __ldcg(reinterpret_cast<const float2 *>(src + DP));
+          v[k] = __ldcg(reinterpret_cast<const float4 *>(src + d));
+        }
+      }
+      float mn = M;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mn = fmaxf(mn, ml[k].x);
+      const float base = mn == -INFINITY ? 0.0f : mn, keep = exp2f(M - base);
+      l *= keep;
+      acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = exp2f(ml[k].x - base);
+        l = fmaf(ml[k].y, w, l);
+        acc.x = fmaf(v[k].x, w, acc.x);
+        acc.y = fmaf(v[k].y, w, acc.y);
+        acc.z = fmaf(v[k].z, w, acc.z);
+        acc.w = fmaf(v[k].w, w, acc.w);
+      }
+      M = mn;
+    }
+    const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+    acc = make_float4(acc.x * scale, acc.y * scale, acc.z * scale, acc.w * scale);
+  }
+  st1<T>(y, 0, acc.x);
+  st1<T>(y, 1, acc.y);
+  st1<T>(y, 2, acc.z);
+  st1<T>(y, 3, acc.w);
+}
+
 int cp_pk(int group) { // heads per CTA
   int pk = 1;
   while (pk < 8 && group % (2 * pk) == 0) pk *= 2;
   return pk;
 }
 
-template <typename T, typename Q>
-int cp_launch(const CUtensorMap &mk, const CUtensorMap &mv, const CpArgs &g, unsigned grid, cudaStream_t st) {
-  if (g.c.D <= 64) {
-    auto kern = cache_attn_prefill<T, Q, 64>;
-    B2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)CpLayout<64>::SMEM));
-    kern<<<grid, CP_THREADS, CpLayout<64>::SMEM, st>>>(mk, mv, g);
-  } else {
-    auto kern = cache_attn_prefill<T, Q, 128>;
-    B2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)CpLayout<128>::SMEM));
-    kern<<<grid, CP_THREADS, CpLayout<128>::SMEM, st>>>(mk, mv, g);
-  }
+template <typename T, typename Q, int DP>
+int cp_launch_dp(const CUtensorMap &mk, const CUtensorMap &mv, const CpArgs &g, int64_t tiles, cudaStream_t st) {
+  auto kern = cache_attn_prefill<T, Q, DP>;
+  B2_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)CpLayout<DP>::SMEM));
+  kern<<<(unsigned)(tiles * g.splits), CP_THREADS, CpLayout<DP>::SMEM, st>>>(mk, mv, g);
   B2_LAUNCH_CHECK();
+  if (g.splits > 1) {
+    cache_attn_prefill_join<T, DP><<<(unsigned)(tiles * (CP_M / 8)), 256, 0, st>>>(g);
+    B2_LAUNCH_CHECK();
+  }
   return B2_OK;
+}
+template <typename T, typename Q>
+int cp_launch(const CUtensorMap &mk, const CUtensorMap &mv, const CpArgs &g, int64_t tiles, cudaStream_t st) {
+  return g.c.D <= 64 ? cp_launch_dp<T, Q, 64>(mk, mv, g, tiles, st) : cp_launch_dp<T, Q, 128>(mk, mv, g, tiles, st);
 }
 
 int cp_read(int reset, const int &symbol) {
@@ -662,18 +759,33 @@ int cp_read(int reset, const int &symbol) {
 
 } // namespace
 
-// CTAs of a call.
-int64_t cache_attn_prefill_ctas(const CaArgs &a) {
+// Query tiles of a call.
+static int64_t cp_tiles(const CaArgs &a) {
   const int pk = cp_pk(a.group), np = CP_M / pk;
   return (int64_t)((a.S + np - 1) / np) * a.B * (a.Hq / pk);
 }
 
-bool cache_attn_prefill_eligible(const CaArgs &a) {
-  return a.D % 16 == 0 && a.D <= 128 && a.T % 16 == 0 && aligned(a.q, 16) && aligned(a.y, 16) && aligned(a.k, 16) &&
-         aligned(a.v, 16) && a.pages > 0 && a.q_h % 8 == 0 && a.q_s % 8 == 0 && cache_attn_prefill_ctas(a) < ((int64_t)1 << 31);
+// CTAs that share a query tile's keys: as many as fill the SMs when the query tiles alone do not, each
+// with at least four tiles of the longest keys the table (and the window) can hold.
+static int cp_splits(const CaArgs &a) {
+  const int64_t tiles = cp_tiles(a);
+  int64_t keys = (int64_t)a.max_pages * a.T;
+  if (a.causal && a.window >= 0) keys = std::min<int64_t>(keys, (int64_t)a.window + a.sinks + 3 * CP_N);
+  const int64_t most = std::min<int64_t>(32, std::max<int64_t>(1, keys / CP_N / 4));
+  return (int)std::max<int64_t>(1, std::min(most, sm_count() / std::max<int64_t>(1, tiles)));
 }
 
-int cache_attn_prefill_launch(const CaArgs &a, bool f16, bool f8, cudaStream_t st) {
+bool cache_attn_prefill_eligible(const CaArgs &a) {
+  return a.D % 16 == 0 && a.D <= 128 && a.T % 16 == 0 && aligned(a.q, 16) && aligned(a.y, 16) && aligned(a.k, 16) &&
+         aligned(a.v, 16) && a.pages > 0 && a.q_h % 8 == 0 && a.q_s % 8 == 0 && cp_tiles(a) < ((int64_t)1 << 31);
+}
+
+size_t cache_attn_prefill_workspace(const CaArgs &a) {
+  const int splits = cp_splits(a);
+  return splits > 1 ? kCounterBytes + (size_t)cp_tiles(a) * splits * CP_M * ((a.D <= 64 ? 64 : 128) + 4) * 4 : 0;
+}
+
+int cache_attn_prefill_launch(const CaArgs &a, bool f16, bool f8, void *ws, cudaStream_t st) {
   CpArgs g{};
   g.c = a;
   g.pk = cp_pk(a.group);
@@ -683,7 +795,9 @@ int cache_attn_prefill_launch(const CaArgs &a, bool f16, bool f8, cudaStream_t s
   g.scale_log2 = a.scale * kLog2E;
   g.div_t = FastDiv((uint32_t)a.T);
   g.chunk = a.T % 128 == 0 ? 128 : a.T % 64 == 0 ? 64 : a.T % 32 == 0 ? 32 : 16;
-  const unsigned grid = (unsigned)cache_attn_prefill_ctas(a);
+  g.splits = cp_splits(a);
+  g.partials = ws ? reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + kCounterBytes) : nullptr;
+  const int64_t tiles = cp_tiles(a);
   // [pages * Hkv][T][D] codes; columns past D read as zeros
   CUtensorMap mk, mv;
   const uint64_t dims[3] = {(uint64_t)a.D, (uint64_t)a.T, (uint64_t)a.pages * a.Hkv};
@@ -691,8 +805,8 @@ int cache_attn_prefill_launch(const CaArgs &a, bool f16, bool f8, cudaStream_t s
   const uint32_t box[3] = {128, (uint32_t)g.chunk, 1};
   if (int rc = make_tensor_map(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   if (int rc = make_tensor_map(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
-  if (f16) return f8 ? cp_launch<__half, Fp8>(mk, mv, g, grid, st) : cp_launch<__half, Int8>(mk, mv, g, grid, st);
-  return f8 ? cp_launch<__nv_bfloat16, Fp8>(mk, mv, g, grid, st) : cp_launch<__nv_bfloat16, Int8>(mk, mv, g, grid, st);
+  if (f16) return f8 ? cp_launch<__half, Fp8>(mk, mv, g, tiles, st) : cp_launch<__half, Int8>(mk, mv, g, tiles, st);
+  return f8 ? cp_launch<__nv_bfloat16, Fp8>(mk, mv, g, tiles, st) : cp_launch<__nv_bfloat16, Int8>(mk, mv, g, tiles, st);
 }
 
 int status_read_cache_attn_prefill(int reset) { return cp_read(reset, g_cache_attn_prefill_status); }
