@@ -184,7 +184,10 @@ extern "C" int b2_cache_attention(const b2_tensor *q, const b2_quantized_cache *
   a.scale = attrs->has_scale ? attrs->scale : 1.0f / sqrtf((float)D);
   a.softcap = attrs->softcap;
   const bool empty = B == 0 || S == 0;
-  const bool prefill = !empty && (int64_t)a.S * a.group > 32 && cache_attn_prefill_eligible(a);
+  // Up to 16 query rows per KV head the split kernel is the faster one, past that the tensor-core kernel
+  // (8 heads, group 4, 6144 keys, us split / prefill: 1 x 4 positions 21 / 25, 1 x 5 33 / 25, 32 x 4
+  // 93 / 134, 32 x 8 217 / 134).
+  const bool prefill = !empty && (int64_t)a.S * a.group > 16 && cache_attn_prefill_eligible(a);
   const bool split = !empty && !prefill && cache_attn_split_eligible(a);
   const int wr = workspace_check(workspace, workspace_bytes,
                                  split ? cache_attn_split_workspace(a) : prefill ? cache_attn_prefill_workspace(a) : 0);

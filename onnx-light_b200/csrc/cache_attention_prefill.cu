@@ -3,8 +3,8 @@
 //
 // Bound: tensor pipe and the exponentials, one of each per score.
 //
-// One CTA owns 128 query rows -- pk heads of one GQA group (pk the largest power of two up to 8 that
-// divides the group) x 128 / pk positions -- and walks the 128-key tiles that any of them sees (the
+// One CTA owns 128 query rows -- pk heads of one GQA group (a power of two that divides it, up to 8 or
+// as few positions leave room for) x 128 / pk positions -- and walks the 128-key tiles that any of them sees (the
 // sinks' tiles, then the window's up to the diagonal):
 //   warp 9     (pages) looks up the tiles' pages and scales ahead of use and brings the codes by TMA,
 //              one box per run of a page's tokens, K and V through two buffers each;
@@ -297,36 +297,41 @@ __global__ void __launch_bounds__(CP_THREADS, 1)
         tc::prefetch_tensormap(&map_v);
       }
       struct Box {
-        int id, row; // page (-1: no token of the sequence), first row in it
+        int id, row; // page as the table has it, first row in it
+        bool live;   // the sequence has tokens there
       };
       auto find = [&](int j) {
-        Box x{-1, 0};
+        Box x{0, 0, false};
         if (j < ntiles) {
           const int key = key0_of(j) + ch * g.chunk;
           if (key < sp.total) {
             const int page = (int)g.div_t.div(key);
             x.id = a.table[(int64_t)b * a.max_pages + page];
             x.row = key - page * a.T;
-            if (x.id < 0 || x.id >= a.pages) {
-              atomicExch(&g_cache_attn_prefill_range, 1);
-              x.id = -1;
-            }
+            x.live = true;
           }
         }
         return x;
       };
-      auto scales = [&](const Box &x) {
-        return x.id >= 0 ? make_float2(a.ks[x.id * a.Hkv + kvh], a.vs[x.id * a.Hkv + kvh]) : make_float2(0.0f, 0.0f);
+      // the page's place among pages and heads, -1 when there is none; reports pages out of range
+      auto place = [&](const Box &x) {
+        if (!x.live) return -1;
+        if (x.id >= 0 && x.id < a.pages) return x.id * a.Hkv + kvh;
+        atomicExch(&g_cache_attn_prefill_range, 1);
+        return -1;
       };
+      auto scales = [&](int z) { return z >= 0 ? make_float2(a.ks[z], a.vs[z]) : make_float2(0.0f, 0.0f); };
       bool ok = true;
       int issued = 0;
       Box x0 = find(my), x1 = find(per + my);
-      float2 s0 = scales(x0);
+      int z0 = place(x0);
+      float2 s0 = scales(z0);
       for (int j0 = 0; ok && j0 < ntiles; j0 += per) {
-        const float2 s1 = scales(x1);
+        const int z1 = place(x1);
+        const float2 s1 = scales(z1);
         const Box x2 = find(j0 + 2 * per + my);
         float4 f = make_float4(0.0f, CP_LV_MIN, 0.0f, 0.0f);
-        if (x0.id >= 0) {
+        if (z0 >= 0) {
           f.x = s0.x * g.scale_log2;
           f.y = fmaxf(log2f(s0.y), CP_LV_MIN); // a NaN gives the bound
           f.z = exp2f(-f.y);
@@ -334,10 +339,10 @@ __global__ void __launch_bounds__(CP_THREADS, 1)
           f.w = f.x > 0.0f && f.x < INFINITY && fabsf(s0.y) < INFINITY ? 1.0f : 2.0f;
           if (!(fabsf(s0.y) < INFINITY)) f.z = __uint_as_float(0x7fc00000u);
         }
-        const bool tiny = x0.id >= 0 && f.y <= CP_LV_MIN;
-        const bool holes = x0.id < 0 || key0_of(min(j0 + my, ntiles - 1)) + (ch + 1) * g.chunk > sp.total;
+        const bool tiny = z0 >= 0 && f.y <= CP_LV_MIN;
+        const bool holes = z0 < 0 || key0_of(min(j0 + my, ntiles - 1)) + (ch + 1) * g.chunk > sp.total;
         const uint32_t tinies = __ballot_sync(0xffffffffu, tiny), holed = __ballot_sync(0xffffffffu, holes);
-        const uint32_t have = __ballot_sync(0xffffffffu, x0.id >= 0);
+        const uint32_t have = __ballot_sync(0xffffffffu, z0 >= 0);
         for (int k = 0; ok && k < per && j0 + k < ntiles; ++k) {
           const int j = j0 + k, s = j & 1;
           if (j >= 2) {
@@ -360,14 +365,14 @@ __global__ void __launch_bounds__(CP_THREADS, 1)
             tc::mbar_expect_tx(&raw_full[2 + s], bytes);
           }
           __syncwarp();
-          if (my == k && x0.id >= 0) {
-            const int z = x0.id * a.Hkv + kvh;
-            tc::tma_load_3d(sm + L::OFF_RAW + s * CP_RAW + ch * box_bytes, &map_k, &raw_full[s], 0, x0.row, z);
-            tc::tma_load_3d(sm + L::OFF_RAW + (2 + s) * CP_RAW + ch * box_bytes, &map_v, &raw_full[2 + s], 0, x0.row, z);
+          if (my == k && z0 >= 0) {
+            tc::tma_load_3d(sm + L::OFF_RAW + s * CP_RAW + ch * box_bytes, &map_k, &raw_full[s], 0, x0.row, z0);
+            tc::tma_load_3d(sm + L::OFF_RAW + (2 + s) * CP_RAW + ch * box_bytes, &map_v, &raw_full[2 + s], 0, x0.row, z0);
           }
           issued = j + 1;
         }
         x0 = x1;
+        z0 = z1;
         x1 = x2;
         s0 = s1;
       }
@@ -539,15 +544,19 @@ __global__ void __launch_bounds__(CP_THREADS, 1)
             bits[w] = below(last_key + 1 - base) & (~below(first_key - base) | below(a.sinks - base));
           }
 #pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[c * 16 + e] *= vk[c];
+          if (a.softcap > 0.0f) { // on its own: its code would be fetched past by every masked tile
+#pragma unroll
+            for (int e = 0; e < 64; ++e) v[e] = a.softcap * tanhf(v[e] * kLn2 / a.softcap) * kLog2E;
+          }
+#pragma unroll
           for (int c = 0; c < 4; ++c) {
             const uint32_t flag = __float_as_uint(sc[(j & 3) * 8 + half * 4 + c].w);
             const uint32_t seen = flag ? (bits[c >> 1] >> ((c & 1) * 16)) & 0xffffu : 0u;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float x = v[c * 16 + e] * vk[c];
-              if (a.softcap > 0.0f) x = a.softcap * tanhf(x * kLn2 / a.softcap) * kLog2E;
-              v[c * 16 + e] = seen >> e & 1u ? x : -INFINITY;
-            }
+            for (int e = 0; e < 16; ++e) v[c * 16 + e] = seen >> e & 1u ? v[c * 16 + e] : -INFINITY;
             poison = poison || (seen != 0u && inv[c] != inv[c]); // it sees values that are not finite
             if (inv[c] != inv[c]) inv[c] = 0.0f;
             vk[c] = 1.0f;
@@ -724,9 +733,12 @@ template <typename T, int DP> __global__ void __launch_bounds__(256) cache_attn_
   st1<T>(y, 3, acc.w);
 }
 
-int cp_pk(int group) { // heads per CTA
-  int pk = 1;
-  while (pk < 8 && group % (2 * pk) == 0) pk *= 2;
+// Heads per CTA: a power of two that divides the group, up to 8, and more where few positions would
+// leave rows empty.
+int cp_pk(const CaArgs &a) {
+  int most = 8, pk = 1;
+  while (most < CP_M && (int64_t)a.S * 2 * most <= CP_M) most *= 2;
+  while (pk < most && a.group % (2 * pk) == 0) pk *= 2;
   return pk;
 }
 
@@ -761,18 +773,28 @@ int cp_read(int reset, const int &symbol) {
 
 // Query tiles of a call.
 static int64_t cp_tiles(const CaArgs &a) {
-  const int pk = cp_pk(a.group), np = CP_M / pk;
+  const int pk = cp_pk(a), np = CP_M / pk;
   return (int64_t)((a.S + np - 1) / np) * a.B * (a.Hq / pk);
 }
 
-// CTAs that share a query tile's keys: as many as fill the SMs when the query tiles alone do not, each
-// with at least four tiles of the longest keys the table (and the window) can hold.
+// CTAs that share a query tile's keys, from the longest the table (and the window) can hold: a key
+// tile takes about 1.3 us, a CTA's start and end 6, the joining kernel 4 and 0.02 per part, and the
+// busiest SM sets the time.  64 queries over 6208 keys (16 query tiles): 84 us with one, 31 with 9.
 static int cp_splits(const CaArgs &a) {
-  const int64_t tiles = cp_tiles(a);
+  const int64_t tiles = cp_tiles(a), sms = sm_count();
   int64_t keys = (int64_t)a.max_pages * a.T;
   if (a.causal && a.window >= 0) keys = std::min<int64_t>(keys, (int64_t)a.window + a.sinks + 3 * CP_N);
-  const int64_t most = std::min<int64_t>(32, std::max<int64_t>(1, keys / CP_N / 4));
-  return (int)std::max<int64_t>(1, std::min(most, sm_count() / std::max<int64_t>(1, tiles)));
+  const double per = 1.3 * (double)((keys + CP_N - 1) / CP_N);
+  int best = 1;
+  double least = 0.0;
+  for (int s = 1; s <= 32 && tiles * (s - 1) < 4 * sms; ++s) {
+    const double cost = (double)((tiles * s + sms - 1) / sms) * (per / s + 6.0) + (s > 1 ? 4.0 + 0.02 * (double)(tiles * s) : 0.0);
+    if (s == 1 || cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
 }
 
 bool cache_attn_prefill_eligible(const CaArgs &a) {
@@ -788,7 +810,7 @@ size_t cache_attn_prefill_workspace(const CaArgs &a) {
 int cache_attn_prefill_launch(const CaArgs &a, bool f16, bool f8, void *ws, cudaStream_t st) {
   CpArgs g{};
   g.c = a;
-  g.pk = cp_pk(a.group);
+  g.pk = cp_pk(a);
   g.np = CP_M / g.pk;
   g.qtiles = (a.S + g.np - 1) / g.np;
   g.hpacks = a.Hq / g.pk;
