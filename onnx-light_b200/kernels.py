@@ -399,7 +399,7 @@ class SwiGLU:
 # ---------------------------------------------------------------------------
 
 
-@dataclass
+@dataclass(slots=True)
 class QuantizedNorm:
     Y: object  # codes: torch.int8, or a QTensor of FLOAT8E4M3FN
     Y_scale: torch.Tensor
@@ -455,13 +455,13 @@ class QuantizedKVCache:
     every layer with the same lengths, then calls :meth:`advance` once.
     """
 
+    __slots__ = ("k", "v", "k_scale", "v_scale", "block_table", "lengths", "dtype")
+
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor,
                  v_scale: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
                  dtype: int):
         if dtype not in (capi.INT8, capi.FLOAT8E4M3FN):
             raise ValueError("QuantizedKVCache: dtype must be INT8 or FLOAT8E4M3FN")
-        if k.element_size() != 1 or v.element_size() != 1:
-            raise ValueError("QuantizedKVCache: k and v must hold 8-bit codes")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.block_table, self.lengths, self.dtype = block_table, lengths, dtype
 
