@@ -113,6 +113,7 @@ extern "C" int b2_scaled_matmul(const b2_tensor *a, const b2_tensor *a_scale, co
   const bool f8 = a->dtype == kF8E4M3FN;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (scaled_skinny_eligible(g, f8)) return scaled_skinny_launch(g, y->dtype, f8, st);
+  if (scaled_pair_eligible(g)) return scaled_pair_launch(g, y->dtype, f8, st);
   if (scaled_tc_eligible(g)) return scaled_tc_launch(g, y->dtype, f8, st);
   if (y->dtype == kFloat16) return launch_any<__half>(g, f8, st);
   if (y->dtype == kBfloat16) return launch_any<__nv_bfloat16>(g, f8, st);

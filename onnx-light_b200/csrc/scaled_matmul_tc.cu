@@ -61,33 +61,6 @@ __device__ __forceinline__ void tile_of(const StArgs &g, int t, int *m, int *n) 
   *m = first + r - *n * height;
 }
 
-// 32 columns of one row: the sums times the row's scale and the columns' (in shared memory).
-template <typename T, typename Q>
-__device__ __forceinline__ void store32(T *y, int left, float as, const float *ws, const uint32_t (&r)[32], bool vec) {
-  float v[32];
-#pragma unroll
-  for (int j = 0; j < 32; j += 4) {
-    const float4 w = *reinterpret_cast<const float4 *>(ws + j);
-    const float f[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      v[j + e] = (std::is_same<Q, Int8>::value ? (float)(int)r[j + e] : __uint_as_float(r[j + e])) * (as * f[e]);
-  }
-  if (vec && left >= 32) {
-#pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      float f[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = v[j + e];
-      Raw8<T>::store(y + j, f);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < left) st1<T>(y, j, v[j]);
-  }
-}
-
 template <typename T, typename Q, int BN, int AR>
 __global__ void __launch_bounds__(ST_THREADS, 1)
     scaled_mm_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
@@ -245,7 +218,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1)
         uint32_t r[32];
         tc::tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * BN + ch * 32), r);
         tc::tmem_ld_wait();
-        if (m < p.M) store32<T, Q>(y + ch * 32, left - ch * 32, as, ws + ch * 32, r, vec);
+        if (m < p.M) store_scaled32<T, Q>(y + ch * 32, left - ch * 32, as, ws + ch * 32, r, vec);
       }
       tc::tc_fence_before();
       __syncwarp();

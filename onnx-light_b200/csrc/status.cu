@@ -32,6 +32,7 @@ int status_read_gemv_c(int reset);
 int status_read_cache_append(int reset);
 int status_read_cache_attention(int reset);
 int status_read_scaled_tc(int reset);
+int status_read_scaled_pair(int reset);
 int status_read_cache_attn_split(int reset);
 int range_read_cache_attn_split(int reset);
 int status_read_cache_attn_prefill(int reset);
@@ -83,7 +84,8 @@ extern "C" B2_API int b2_kernel_status(int reset) {
                       {"b200::QuantizedCacheAttention", range_read_cache_attn_prefill, kCacheRange},
                       {"cache_attn_split", status_read_cache_attn_split, 0},
                       {"cache_attn_prefill", status_read_cache_attn_prefill, 0},
-                      {"scaled_mm_tc", status_read_scaled_tc, 0}};
+                      {"scaled_mm_tc", status_read_scaled_tc, 0},
+                      {"scaled_mm_pair", status_read_scaled_pair, 0}};
   int first = 0;
   for (const Src &s : srcs) {
     const int v = s.read(reset);

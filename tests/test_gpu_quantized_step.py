@@ -199,6 +199,19 @@ def test_product(b2, m, k, n, codes):
         check_product(b2, a, as_, w, ws, t, codes)
 
 
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("m,k,n", [(2500, 400, 4000), (2561, 1040, 4001), (300, 144, 19000), (9000, 4096, 1300),
+                                   (38000, 16, 250)])
+def test_product_large(b2, m, k, n, codes):
+    """Outputs of several hundred tiles: last tiles cut in both directions, several rounds of tiles."""
+    g = gen(m + n)
+    a, w = operand(g, codes, m, k), operand(g, codes, n, k)
+    as_ = torch.rand(m, generator=g, device="cuda") * 0.01 + 0.001
+    ws = torch.rand(n, generator=g, device="cuda") * 0.001 + 0.0001
+    for t in (torch.float16, torch.bfloat16, torch.float32):
+        check_product(b2, a, as_, w, ws, t, codes)
+
+
 @pytest.mark.parametrize("m", [1, 40, 130])
 def test_product_one_scale_and_shapes(b2, m):
     g = gen(m)
