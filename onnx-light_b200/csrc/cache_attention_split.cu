@@ -181,6 +181,18 @@ __device__ __forceinline__ bool cs_live(const CsArgs &g, const CsSeq &s, int fir
   return g.c.window < 0 || key0 + KEYS > first - g.c.window || key0 < g.c.sinks;
 }
 
+// Sum of v over the lanes before this one, and over the warp.
+__device__ __forceinline__ int warp_scan(int v, int *total) {
+  const int lane = threadIdx.x & 31;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += t;
+  }
+  *total = __shfl_sync(0xffffffffu, inc, 31);
+  return inc - v;
+}
 // Sum of v over the block and the sum over the threads before this one; every thread calls it.
 template <int THREADS> __device__ __forceinline__ int block_scan(int v, int *total, int *red) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -242,15 +254,23 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
     tc::fence_barrier_init();
   }
   // ---- this CTA's range of units ----
+  // Up to 32 sequences every warp works it out for itself, a lane for a sequence; up to a block's
+  // threads the block does, a thread for a sequence; past that it takes them in runs.
+  const bool by_warp = a.B <= 32, at_once = a.B <= L::THREADS;
+  const int me = by_warp ? lane : threadIdx.x;
+  auto scan = [&](int v, int *total) { // sum of v before this sequence, and over all
+    return by_warp ? warp_scan(v, total) : block_scan<L::THREADS>(v, total, misc);
+  };
   bool bad = false;
-  int tiles_all = 0, mine = 0, before = 0; // all sequences'; with B <= THREADS, of sequence threadIdx.x
+  int tiles_all = 0, before = 0; // all sequences' tiles (per pair); those before sequence `me`
+  CsSeq mine{};                  // sequence `me`, when all are looked at at once
   for (int b0 = 0; b0 < a.B; b0 += L::THREADS) {
-    const int b = b0 + threadIdx.x;
+    const int b = b0 + me;
     bool bb = false;
-    mine = b < a.B ? cs_seq(a, b, &bb).tiles : 0;
+    mine = b < a.B ? cs_seq(a, b, &bb) : CsSeq{};
     bad |= bb;
     int t;
-    before = block_scan<L::THREADS>(mine, &t, misc);
+    before = scan(mine.tiles, &t);
     tiles_all += t;
   }
   if (bad) atomicExch(&g_cache_attn_split_range, 1);
@@ -261,55 +281,83 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
   int u0 = cta * share + min(cta, extra), u1 = u0 + share + (cta < extra);
   // With few pairs, CTAs of one pair each where that costs at most a quarter more units per CTA: a CTA
   // on a boundary would do two pairs' work and merges one after the other (for 8 pairs of 129 tiles
-  // it finished at 21 us, the others at 8).
+  // it finished at 21 us, the others at 8).  The fewest units per CTA that will do, by bisection.
   bool own_pair = false;
-  int own_first = 0, own_count = 0; // the pair's CTAs
-  if (a.B <= L::THREADS && a.B * hp <= G && !g.align_pairs) {
-    const int q0 = (U + G - 1) / G;
-    for (int q = q0; q <= q0 + max(1, q0 / 4) && !own_pair; ++q) {
-      const int parts = (mine + q - 1) / q;
+  int parts = 0, at = 0;            // CTAs per pair of sequence `me`, its first CTA
+  int own_first = 0, own_count = 0; // the CTAs of this CTA's pair
+  if (at_once && a.B * hp <= G && !g.align_pairs) {
+    int lo = (U + G - 1) / G, hi = lo + max(1, lo / 4);
+    auto fits = [&](int q) {
+      parts = (mine.tiles + q - 1) / q;
       int all;
-      const int at = block_scan<L::THREADS>(parts, &all, misc) * hp;
-      if (all * hp > G) continue;
+      at = scan(parts, &all) * hp;
+      own_count = all * hp;
+      return own_count <= G;
+    };
+    own_pair = fits(lo);
+    if (!own_pair && fits(hi)) {
       own_pair = true;
-      if (cta >= all * hp) return;
-      if (mine && cta >= at && cta < at + parts * hp) {
-        misc[16] = threadIdx.x;
-        misc[17] = before;
-        misc[18] = at;
-        misc[19] = parts;
+      ++lo;
+      bool last = true; // whether parts and at are those of hi
+      while (lo < hi) {
+        const int q = (lo + hi) / 2;
+        last = fits(q);
+        if (last) hi = q;
+        else lo = q + 1;
       }
+      if (!last) fits(hi);
     }
+    if (own_pair && cta >= own_count) return;
   }
-  if (!own_pair) {
-    if (a.B <= L::THREADS) {
-      if (mine && u0 >= before * hp && u0 < (before + mine) * hp) {
-        misc[16] = threadIdx.x;
-        misc[17] = before;
-      }
-    } else {
-      int run = 0;
-      for (int b0 = 0; b0 < a.B; b0 += L::THREADS) {
-        const int b = b0 + threadIdx.x;
-        bool bb;
-        const int n = b < a.B ? cs_seq(a, b, &bb).tiles : 0;
-        int t;
-        const int at = run + block_scan<L::THREADS>(n, &t, misc);
-        run += t;
-        if (n && u0 >= at * hp && u0 < (at + n) * hp) {
-          misc[16] = b;
-          misc[17] = at;
-        }
-      }
-    }
-  }
-  __syncthreads();
   CsWalk walk;
-  walk.b = misc[16];
-  walk.before = misc[17];
-  walk.s = cs_seq(a, walk.b, &bad);
+  if (at_once) {
+    const bool here = mine.tiles && (own_pair ? cta >= at && cta < at + parts * hp
+                                              : u0 >= before * hp && u0 < (before + mine.tiles) * hp);
+    if (by_warp) {
+      const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+      walk.b = src;
+      walk.before = __shfl_sync(0xffffffffu, before, src);
+      at = __shfl_sync(0xffffffffu, at, src);
+      parts = __shfl_sync(0xffffffffu, parts, src);
+      walk.s.sp.past = __shfl_sync(0xffffffffu, mine.sp.past, src);
+      walk.s.sp.count = __shfl_sync(0xffffffffu, mine.sp.count, src);
+      walk.s.sp.total = __shfl_sync(0xffffffffu, mine.sp.total, src);
+      walk.s.first = __shfl_sync(0xffffffffu, mine.first, src);
+      walk.s.sink_tiles = __shfl_sync(0xffffffffu, mine.sink_tiles, src);
+      walk.s.tiles = __shfl_sync(0xffffffffu, mine.tiles, src);
+    } else if (here) {
+      misc[16] = threadIdx.x;
+      misc[17] = before;
+      misc[18] = at;
+      misc[19] = parts;
+    }
+  } else {
+    int run = 0;
+    for (int b0 = 0; b0 < a.B; b0 += L::THREADS) {
+      const int b = b0 + threadIdx.x;
+      bool bb;
+      const int n = b < a.B ? cs_seq(a, b, &bb).tiles : 0;
+      int t;
+      const int first = run + block_scan<L::THREADS>(n, &t, misc);
+      run += t;
+      if (n && u0 >= first * hp && u0 < (first + n) * hp) {
+        misc[16] = b;
+        misc[17] = first;
+      }
+    }
+  }
+  __syncthreads(); // the barriers, and what another thread found
+  if (!by_warp) {
+    walk.b = misc[16];
+    walk.before = misc[17];
+    walk.s = cs_seq(a, walk.b, &bad);
+    if (own_pair) {
+      at = misc[18];
+      parts = misc[19];
+    }
+  }
   if (own_pair) {
-    const int at = misc[18], parts = misc[19], pair = (cta - at) / parts, part = cta - at - pair * parts;
+    const int pair = (cta - at) / parts, part = cta - at - pair * parts;
     own_first = cta - part;
     own_count = parts;
     const int n = walk.s.tiles, first = walk.before * hp + pair * n, q = n / parts, x = n - q * parts;
