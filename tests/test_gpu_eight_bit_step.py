@@ -565,6 +565,27 @@ def test_attention_not_finite_values_stay_where_they_are_seen(b2, rows, codes, h
         sc.copy_(keep)
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_cache_past_4_gib(b2, rows):
+    """Pages whose codes lie past 2^32 bytes of their pool, for the append and both tensor-core kernels."""
+    pages, heads, page, head = 66000, 8, 64, 128  # 4.3e9 bytes each of K and V
+    cache = b2.QuantizedKVCache.allocate(1, heads, 128, head, page_size=page, dtype=b2.INT8, pages=pages,
+                                         block_table=torch.tensor([[pages - 1, pages - 2]], dtype=torch.int32,
+                                                                  device="cuda"))
+    assert cache.k.numel() > 1 << 32
+    kv = torch.randn(2, 1, heads, 100, head, generator=gen(1), device="cuda").half()
+    b2.KVCacheAppend()(kv[0], kv[1], cache)
+    cache.advance(100)
+    for pool, x in ((cache.k, kv[0]), (cache.v, kv[1])):
+        got = values(pool[pages - 1]) * cache.k_scale[pages - 1].double()[:, None, None] if pool is cache.k else \
+            values(pool[pages - 1]) * cache.v_scale[pages - 1].double()[:, None, None]
+        step = (cache.k_scale if pool is cache.k else cache.v_scale)[pages - 1].double()[:, None, None]
+        assert bool(((got - x[0, :, :64].double()).abs() <= 0.501 * step).all())
+    cache.lengths.fill_(100 - rows)
+    q = torch.randn(1, 16, rows, head, generator=gen(2), device="cuda").half()
+    check_attention(b2, cache, q)
+
+
 def test_attention_identical_runs(b2):
     """The same call twice gives the same bits, whatever order blocks finish in."""
     for past, rows in (([3000, 17, 900], 1), ([2500], 3), ([600], 500)):
