@@ -9,7 +9,9 @@
 // it in registers between the three steps (statistic, largest magnitude, codes), so x and the
 // residual are read once and nothing is read back.  The norm is taken of the unrounded sum.  All
 // sums are fp32 in a fixed order; the maxima are integer maxima of magnitudes, which keep a NaN.
-// Codes come from a correctly rounded division, the same quotient an unfused chain computes.
+// n itself is never formed: 1 / sqrt(...) is split into a power of two, which scales h exactly, and a
+// rest in [1, 2) that only the scale takes, so a code is h w over the largest h w and carries the
+// rounding of h w and of the quotient alone.
 #include "quant8.cuh"
 
 namespace b2 {
@@ -38,6 +40,54 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+
+// 1 / sqrt(mean + epsilon) as p2 * rest: p2 a power of two, 1 <= rest < 2 (0, infinity and NaN are p2).
+struct Rms {
+  float p2, rest;
+  __device__ __forceinline__ Rms(float ss, int width, float eps) {
+    const float r = 1.0f / sqrtf(ss / (float)width + eps);
+    const uint32_t u = __float_as_uint(r);
+    const bool split = r > 0.0f && r < INFINITY; // never subnormal: a root is at most 2^64
+    p2 = split ? __uint_as_float(u & 0x7f800000u) : r;
+    rest = split ? __uint_as_float((u & 0x007fffffu) | 0x3f800000u) : 1.0f;
+  }
+};
+template <typename Q> __device__ __forceinline__ float scale_of(uint32_t top, float rest) {
+  return __fdiv_rn(__uint_as_float(top) * rest, Code<Q>::kMax);
+}
+
+// Quotients by top / 127 or 448, kept as the sum of two floats: q = v inv is within some ulps,
+// v - q (hi + lo) comes from two FMAs, and q + that * inv is the quotient rounded once, but for a
+// second-order term.  A ratio next to a tie between two codes so falls on the side where the inputs
+// put it.  Zeros where the group's scale is 0, infinite or not a number.
+template <typename Q> struct ByTop {
+  float hi, lo, inv;
+  int kind; // 0 zeros, 1 products, 2 divisions
+  __device__ __forceinline__ ByTop(uint32_t top, float rest) {
+    const float t = __uint_as_float(top), s = scale_of<Q>(top, rest);
+    hi = __fdiv_rn(t, Code<Q>::kMax);
+    kind = !(s > 0.0f && s < INFINITY) ? 0 : hi > 1e-25f && hi < 1e30f ? 1 : 2;
+    lo = fmaf(-hi, Code<Q>::kMax, t) * (1.0f / Code<Q>::kMax);
+    inv = kind == 1 ? __frcp_rn(hi) : 0.0f;
+  }
+  __device__ __forceinline__ float one(float v) const {
+    if (kind != 1) return kind == 0 ? 0.0f : __fdiv_rn(v, hi);
+    const float q = v * inv;
+    return fmaf(fmaf(-q, lo, fmaf(-q, hi, v)), inv, q);
+  }
+  __device__ __forceinline__ void divide(float (&v)[8]) const {
+    if (kind == 1) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float q = v[e] * inv;
+        v[e] = fmaf(fmaf(-q, lo, fmaf(-q, hi, v[e])), inv, q);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = one(v[e]);
+    }
+  }
+};
 
 // Groups of columns: kRow one group per row; kLanes a group is 8 * seg columns with seg a power
 // of two up to 32, so it lies in seg neighbouring lanes of one warp; kShared any other multiple
@@ -88,7 +138,7 @@ __global__ void __launch_bounds__(1024) rms_norm_q_vec(const RnqArgs a) {
     }
   }
   ss = block_sum(ss, red_f);
-  const float r = 1.0f / sqrtf(ss / (float)a.width + a.eps);
+  const Rms r(ss, a.width, a.eps);
   uint32_t m[KV];
 #pragma unroll
   for (int k = 0; k < KV; ++k) {
@@ -98,28 +148,36 @@ __global__ void __launch_bounds__(1024) rms_norm_q_vec(const RnqArgs a) {
       wr[k].get(w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        h[k][e] = h[k][e] * r * w[e];
+        h[k][e] = h[k][e] * r.p2 * w[e];
         m[k] = max(m[k], mag(h[k][e]));
       }
     }
   }
-  float s[KV];
+  // m: the largest magnitude of the group that vector k lies in
   if (MODE == kRow) {
     uint32_t mm = 0u;
 #pragma unroll
     for (int k = 0; k < KV; ++k) mm = max(mm, m[k]);
-    const float sc = __fdiv_rn(__uint_as_float(block_max(mm, red_u)), Code<Q>::kMax);
-    if (tid == 0) a.y_scale[row] = sc;
+    mm = block_max(mm, red_u);
+    if (tid == 0) a.y_scale[row] = scale_of<Q>(mm, r.rest);
+    const ByTop<Q> by(mm, r.rest);
 #pragma unroll
-    for (int k = 0; k < KV; ++k) s[k] = sc;
-  } else if (MODE == kLanes) {
+    for (int k = 0; k < KV; ++k) {
+      const int v = tid + k * nt;
+      if (v < nv) {
+        by.divide(h[k]);
+        *reinterpret_cast<uint2 *>(a.y + base + 8 * v) = enc8<Q>(h[k]);
+      }
+    }
+    return;
+  }
+  if (MODE == kLanes) {
     const int seg = a.group >> 3;
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
       for (int o = seg >> 1; o; o >>= 1) m[k] = max(m[k], __shfl_xor_sync(0xffffffffu, m[k], o));
-      s[k] = __fdiv_rn(__uint_as_float(m[k]), Code<Q>::kMax);
       const int v = tid + k * nt;
-      if (v < nv && v % seg == 0) a.y_scale[row * a.groups + v / seg] = s[k];
+      if (v < nv && v % seg == 0) a.y_scale[row * a.groups + v / seg] = scale_of<Q>(m[k], r.rest);
     }
   } else {
     // gmax was cleared before block_sum's barrier
@@ -128,18 +186,16 @@ __global__ void __launch_bounds__(1024) rms_norm_q_vec(const RnqArgs a) {
       if (tid + k * nt < nv) atomicMax(&gmax[(8 * (tid + k * nt)) / a.group], m[k]);
     __syncthreads();
     for (int g = tid; g < a.groups; g += nt)
-      a.y_scale[row * a.groups + g] = __fdiv_rn(__uint_as_float(gmax[g]), Code<Q>::kMax);
+      a.y_scale[row * a.groups + g] = scale_of<Q>(gmax[g], r.rest);
 #pragma unroll
     for (int k = 0; k < KV; ++k)
-      s[k] = tid + k * nt < nv
-                 ? __fdiv_rn(__uint_as_float(gmax[(8 * (tid + k * nt)) / a.group]), Code<Q>::kMax)
-                 : 0.0f;
+      if (tid + k * nt < nv) m[k] = gmax[(8 * (tid + k * nt)) / a.group];
   }
 #pragma unroll
   for (int k = 0; k < KV; ++k) {
     const int v = tid + k * nt;
     if (v < nv) {
-      Divisor(s[k]).divide(h[k]);
+      ByTop<Q>(m[k], r.rest).divide(h[k]);
       *reinterpret_cast<uint2 *>(a.y + base + 8 * v) = enc8<Q>(h[k]);
     }
   }
@@ -162,18 +218,17 @@ __global__ void __launch_bounds__(256) rms_norm_q_any(const RnqArgs a) {
     ss = fmaf(v, v, ss);
   }
   ss = block_sum(ss, red_f);
-  const float r = 1.0f / sqrtf(ss / (float)a.width + a.eps);
+  const Rms r(ss, a.width, a.eps);
   for (int c = threadIdx.x; c < a.width; c += 256) {
-    const float v = hs[c] * r * ld1<T>(a.w, c);
+    const float v = hs[c] * r.p2 * ld1<T>(a.w, c);
     hs[c] = v;
     atomicMax(&gmax[c / a.group], mag(v));
   }
   __syncthreads();
   for (int g = threadIdx.x; g < a.groups; g += 256)
-    a.y_scale[row * a.groups + g] = __fdiv_rn(__uint_as_float(gmax[g]), Code<Q>::kMax);
+    a.y_scale[row * a.groups + g] = scale_of<Q>(gmax[g], r.rest);
   for (int c = threadIdx.x; c < a.width; c += 256)
-    a.y[base + c] = (uint8_t)Code<Q>::enc(
-        __fdiv_rn(hs[c], __fdiv_rn(__uint_as_float(gmax[c / a.group]), Code<Q>::kMax)));
+    a.y[base + c] = (uint8_t)Code<Q>::enc(ByTop<Q>(gmax[c / a.group], r.rest).one(hs[c]));
 }
 
 constexpr int kMaxShared = 220 * 1024;
