@@ -1,7 +1,8 @@
 // The scaled 8-bit product (b2_scaled_matmul) on tcgen05 tensor cores: prompts and batches.
 //
-// Bound: tensor pipe for prompts.  A tile is 128 rows of A by BN rows of W; both are K-major, so one
-// 128-byte-wide TMA box each (128-byte swizzle) feeds kind::i8 or kind::f8f6f4 with K = 32 a step.
+// Bound: tensor pipe for prompts, the ring's loads for few rows.  K = 4096, FLOAT8, in a graph: 32 x 11008
+// outputs 10.7 us, 4.2 TB/s; 512 x 9472 18.7 us, 2130 TFLOP/s.
+// A tile is 128 rows of A by BN rows of W; both are K-major, so one 128-byte-wide TMA box each (128-byte swizzle) feeds kind::i8 or kind::f8f6f4 with K = 32 a step.
 // Persistent CTAs, one per SM, 192 threads:
 //   warp 0     TMA producer: a ring of [128 + BN] x 128-byte stages that runs on across tiles;
 //   warp 1     MMA issuer: BN columns of TMEM per tile, two buffers, so the next tile's sums start
@@ -79,7 +80,8 @@ __global__ void __launch_bounds__(ST_THREADS, 1)
   const SmArgs &p = g.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = g.mt * g.nt, kt_count = (int)((p.K + L::KB * ST_BK - 1) / (L::KB * ST_BK));
-  constexpr uint32_t COLS = 2 * BN < 32 ? 32 : 2 * BN;
+  constexpr uint32_t BUF = BN <= 32 ? 32 : BN <= 64 ? 64 : BN <= 128 ? 128 : 256; // columns per buffer of sums
+  constexpr uint32_t COLS = 2 * BUF;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -166,8 +168,8 @@ __global__ void __launch_bounds__(ST_THREADS, 1)
             for (int kk = 0; kk < ST_BK / 32; ++kk) {
               const uint64_t ad = a0 + at + kb * (L::A >> 4) + kk * 2, wd = w0 + at + kb * (L::W >> 4) + kk * 2;
               const uint32_t more = (kt > 0 || kb > 0 || kk > 0) ? 1u : 0u;
-              if constexpr (std::is_same<Q, Int8>::value) tc::mma_i8(tmem + b * BN, ad, wd, id, more);
-              else mma_f8(tmem + b * BN, ad, wd, id, more);
+              if constexpr (std::is_same<Q, Int8>::value) tc::mma_i8(tmem + b * BUF, ad, wd, id, more);
+              else mma_f8(tmem + b * BUF, ad, wd, id, more);
             }
           tc::tc_commit(&empty[s]);
           if (++s == L::STAGES) {
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1)
       for (int ch = 0; ch < BN / 32; ++ch) {
         if (ch * 32 >= left) break;
         uint32_t r[32];
-        tc::tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * BN + ch * 32), r);
+        tc::tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * BUF + ch * 32), r);
         tc::tmem_ld_wait();
         if (m < p.M) store_scaled32<T, Q>(y + ch * 32, left - ch * 32, as, ws + ch * 32, r, vec);
       }
@@ -243,9 +245,18 @@ int launch(const CUtensorMap &ma, const CUtensorMap &mw, const StArgs &g, cudaSt
 
 template <typename T, typename Q>
 int pick(int bn, int ar, const CUtensorMap &ma, const CUtensorMap &mw, const StArgs &g, cudaStream_t st) {
-  if (bn == 256) return ar == 32 ? launch<T, Q, 256, 32>(ma, mw, g, st) : launch<T, Q, 256, 128>(ma, mw, g, st);
-  if (bn == 128) return ar == 32 ? launch<T, Q, 128, 32>(ma, mw, g, st) : launch<T, Q, 128, 128>(ma, mw, g, st);
-  if (bn == 64) return ar == 32 ? launch<T, Q, 64, 32>(ma, mw, g, st) : launch<T, Q, 64, 128>(ma, mw, g, st);
+  switch (bn) {
+#define B2_WIDTH(BN)                                                                                                    \
+  case BN:                                                                                                             \
+    return ar == 32 ? launch<T, Q, BN, 32>(ma, mw, g, st) : launch<T, Q, BN, 128>(ma, mw, g, st)
+    B2_WIDTH(256);
+    B2_WIDTH(192);
+    B2_WIDTH(160);
+    B2_WIDTH(128);
+    B2_WIDTH(96);
+    B2_WIDTH(64);
+#undef B2_WIDTH
+  }
   return ar == 32 ? launch<T, Q, 32, 32>(ma, mw, g, st) : launch<T, Q, 32, 128>(ma, mw, g, st);
 }
 
@@ -263,10 +274,12 @@ int scaled_tc_launch(const SmArgs &p, int y_dtype, bool f8, cudaStream_t st) {
   g.mt = (int)((p.M + ST_BM - 1) / ST_BM);
   // Tile width: a tile's time grows like its width plus a fixed part (K = 4096, one tile per SM: 4.4,
   // 5.0, 8 and 11 us past the launch for 32, 64, 128 and 256 columns), and the busiest SM sets the
-  // call's.  32 x 11008 outputs: 16.6, 14.6, 12.3 and 16.6 us with 3, 2, 1 and 1 tiles on it.
+  // call's.  32 x 11008 outputs: 16.6, 14.6, 12.3 and 16.6 us with 3, 2, 1 and 1 tiles on it.  The widths
+  // between the powers of two fill a last round: 200 x 11008 16.7 -> 13.0 us (192 columns), 600 x 4096
+  // 15.8 -> 12.4 (160), 512 x 11008 29.1 -> 22.3 (160), 128 x 11008 11.9 -> 11.4 (96).
   int bn = 256;
   int64_t best = INT64_MAX;
-  for (int w = 256; w >= 32; w /= 2) {
+  for (const int w : {256, 192, 160, 128, 96, 64, 32}) {
     const int64_t tiles = g.mt * ((p.N + w - 1) / w), cost = (tiles + sm_count() - 1) / sm_count() * (w + 96);
     if (cost < best) {
       best = cost;

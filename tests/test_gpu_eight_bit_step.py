@@ -212,6 +212,19 @@ def test_product_large(b2, m, k, n, codes):
         check_product(b2, a, as_, w, ws, t, codes)
 
 
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("m,k,n", [(32, 272, 11008), (128, 272, 11001), (600, 144, 4096), (577, 144, 4090), (200, 400, 11008),
+                                   (129, 400, 11000), (512, 144, 11008), (1500, 80, 4097)])
+def test_product_between_powers_of_two(b2, m, k, n, codes):
+    """Sizes that tiles of 96, 160 and 192 columns fit better, also with a cut last tile."""
+    g = gen(m + 3 * n)
+    a, w = operand(g, codes, m, k), operand(g, codes, n, k)
+    as_ = torch.rand(m, generator=g, device="cuda") * 0.01 + 0.001
+    ws = torch.rand(n, generator=g, device="cuda") * 0.001 + 0.0001
+    for t in (torch.float16, torch.bfloat16, torch.float32):
+        check_product(b2, a, as_, w, ws, t, codes)
+
+
 @pytest.mark.parametrize("m", [1, 40, 130])
 def test_product_one_scale_and_shapes(b2, m):
     g = gen(m)
