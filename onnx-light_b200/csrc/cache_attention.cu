@@ -8,8 +8,8 @@
 // cache_attn_any: one warp owns one (sequence, query head, query).  32 keys at a time each lane
 // scores one key (fp32), the warp keeps a running maximum and sum, and the lanes then own the head's
 // columns for P.V.  It reads a key's codes byte by byte and shares nothing between the heads of a
-// group: right for any head size, page size and alignment, bound by its own loads (32 sequences of 8192
-// tokens, 32 / 8 heads of 128, pages of 12: 15.7 ms).
+// group: right for any head size, page size and alignment, bound by its own loads (32 sequences of up to
+// 8192 tokens, 32 / 8 heads of 128, pages of 12: 15.7 ms).
 #include "cache_attention.cuh"
 
 namespace b2 {
