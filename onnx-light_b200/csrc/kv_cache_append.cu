@@ -35,24 +35,31 @@ struct KaArgs {
   int64_t s_b, s_h, s_s; // strides (elements) of the new tokens over batch, head, position
   int64_t pages;
   int B, H, S, T, D, max_pages, slots;
+  FastDiv div_t, div_h, div_slots, div_row; // by T, H, slots, vectors (or values) in a row
 };
+
+// Four codes times the ratio of the old scale to the new one.
+template <typename Q> __device__ __forceinline__ uint32_t rescale4(uint32_t c, float ratio) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    r |= Code<Q>::enc(__fmul_rn(Code<Q>::dec((c >> (8 * e)) & 0xffu), ratio)) << (8 * e);
+  return r;
+}
 
 template <typename T, typename Q, bool VEC>
 __global__ void __launch_bounds__(KA_THREADS) kv_cache_append_kernel(const KaArgs a) {
   __shared__ uint32_t red[32];
-  int64_t u = blockIdx.x;
-  const int side = (int)(u & 1);
-  u >>= 1;
-  const int h = (int)(u % a.H);
-  u /= a.H;
-  const int slot = (int)(u % a.slots), b = (int)(u / a.slots);
+  const int side = (int)(blockIdx.x & 1);
+  const uint32_t u = blockIdx.x >> 1, uh = a.div_h.div(u), ub = a.div_slots.div(uh);
+  const int h = (int)(u - uh * a.H), slot = (int)(uh - ub * a.slots), b = (int)ub;
   int64_t past = a.lengths[b];
   int64_t n = a.counts ? a.counts[b] : a.S;
   const int64_t room = (int64_t)a.max_pages * a.T;
   bool bad = past < 0 || n < 0 || n > a.S || past + n > room;
   past = max(past, (int64_t)0);
   n = min(min(max(n, (int64_t)0), (int64_t)a.S), room - past);
-  const int64_t page = past / a.T + slot; // place in the table
+  const int64_t page = (int64_t)a.div_t.div((uint32_t)past) + slot; // place in the table
   const int64_t lo = max(past, page * a.T), hi = min(past + n, (page + 1) * a.T);
   if (lo >= hi) {
     if (bad && threadIdx.x == 0) atomicExch(&g_cache_append_status, 1);
@@ -65,7 +72,7 @@ __global__ void __launch_bounds__(KA_THREADS) kv_cache_append_kernel(const KaArg
                  (lo - past) * a.s_s;
   const int dv = VEC ? a.D >> 3 : a.D, nv = rows * dv;
   auto at = [&](int v) { // element offset of vector (or value) v of the new rows
-    const int r = v / dv;
+    const int r = (int)a.div_row.div((uint32_t)v);
     return (int64_t)r * a.s_s + (int64_t)(v - r * dv) * (VEC ? 8 : 1);
   };
   Raw8<T> held[KA_HELD];
@@ -105,8 +112,25 @@ __global__ void __launch_bounds__(KA_THREADS) kv_cache_append_kernel(const KaArg
   // ---- the older tokens of a page whose scale grew ----
   if (s > before && older) {
     const float ratio = __fdiv_rn(before, s);
-    for (int i = threadIdx.x; i < older * a.D; i += KA_THREADS)
-      dst[i] = (uint8_t)Code<Q>::enc(__fmul_rn(Code<Q>::dec(dst[i]), ratio));
+    if constexpr (VEC) { // four vectors in flight a thread: one by one each waits for the last's store
+      const int no = older * dv;
+      for (int i = threadIdx.x; i < no; i += 4 * KA_THREADS) {
+        uint2 c[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i + k * KA_THREADS < no) c[k] = reinterpret_cast<const uint2 *>(dst)[i + k * KA_THREADS];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i + k * KA_THREADS < no) {
+            c[k].x = rescale4<Q>(c[k].x, ratio);
+            c[k].y = rescale4<Q>(c[k].y, ratio);
+            reinterpret_cast<uint2 *>(dst)[i + k * KA_THREADS] = c[k];
+          }
+      }
+    } else {
+      for (int i = threadIdx.x; i < older * a.D; i += KA_THREADS)
+        dst[i] = (uint8_t)Code<Q>::enc(__fmul_rn(Code<Q>::dec(dst[i]), ratio));
+    }
   }
   // ---- the new codes ----
   dst += (int64_t)older * a.D;
@@ -247,6 +271,10 @@ extern "C" int b2_kv_cache_append(const b2_tensor *k, const b2_tensor *v,
                    q8::aligned(cache->k->data, 8) && q8::aligned(cache->v->data, 8);
   const bool f8 = cache->k->dtype == kF8E4M3FN;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  a.div_t = FastDiv((uint32_t)a.T);
+  a.div_h = FastDiv((uint32_t)a.H);
+  a.div_slots = FastDiv((uint32_t)a.slots);
+  a.div_row = FastDiv((uint32_t)(vec ? D / 8 : D));
   if (k->dtype == kFloat16) return launch<__half>(a, f8, vec, (unsigned)grid, st);
   if (k->dtype == kBfloat16) return launch<__nv_bfloat16>(a, f8, vec, (unsigned)grid, st);
   return launch<float>(a, f8, vec, (unsigned)grid, st);
