@@ -12,7 +12,7 @@
 // scale; a page's values stay in registers between the maximum and the codes when there are at
 // most 8192 of them (64 tokens of 128), and are read again (from cache) past that.
 // Measured (8 heads of 128, pages of 64, FLOAT8): prompts of 4 ragged sequences of up to 2048 BFLOAT16
-// tokens 16.4 us, 2.3 TB/s; one token for each of 32 sequences 3.6 us in a graph.
+// tokens 12.5 us, 3.1 TB/s; one token for each of 32 sequences 3.7 us in a graph.
 #include "quant8.cuh"
 
 namespace b2 {
@@ -24,8 +24,10 @@ namespace {
 
 using namespace q8;
 
-constexpr int KA_THREADS = 256;
-constexpr int KA_HELD = 4; // vectors of 8 values a thread keeps in registers
+// Threads x vectors of 8 values that a thread keeps in registers.  128 x 8, 256 x 4 and 64 x 16 take the
+// prompts above 8.8, 10.7 and 11.4 us in a graph, pages of 16 tokens 21, 28 and 19, of 256 tokens 15, 13 and 23.
+constexpr int KA_THREADS = 128;
+constexpr int KA_HELD = 8;
 
 struct KaArgs {
   const void *src[2];
