@@ -19,7 +19,7 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// Element-wise a * b + c, a + b and a - b on two fp32 lanes (one packed
+// Element-wise a * b + c, a * b, a + b and a - b on two fp32 lanes (one packed
 // instruction each on sm_100; the same IEEE operation per element).
 __device__ __forceinline__ uint64_t f2pack(float x, float y) {
   uint64_t r;
@@ -34,6 +34,11 @@ __device__ __forceinline__ float2 f2unpack(uint64_t r) {
 __device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 __device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {

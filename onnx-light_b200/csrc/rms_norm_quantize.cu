@@ -14,6 +14,7 @@
 // rounding of h w and of the quotient alone.
 // Measured: 8192 x 4096 BFLOAT16 with residual and FLOAT8 codes 45 us, 5.2 TB/s; one such row 2.4 us
 // in a graph.
+#include "attn_math.cuh"
 #include "quant8.cuh"
 
 namespace b2 {
@@ -41,6 +42,12 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+__device__ __forceinline__ void unpack2(uint64_t v, float &x, float &y) {
+  const float2 f = f2unpack(v);
+  x = f.x;
+  y = f.y;
 }
 
 // 1 / sqrt(mean + epsilon) as p2 * rest: p2 a power of two, 1 <= rest < 2 (0, infinity and NaN are p2).
@@ -79,10 +86,11 @@ template <typename Q> struct ByTop {
   }
   __device__ __forceinline__ void divide(float (&v)[8]) const {
     if (kind == 1) {
+      const uint64_t i2 = f2pack(inv, inv), h2 = f2pack(-hi, -hi), l2 = f2pack(-lo, -lo);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float q = v[e] * inv;
-        v[e] = fmaf(fmaf(-q, lo, fmaf(-q, hi, v[e])), inv, q);
+      for (int e = 0; e < 8; e += 2) {
+        const uint64_t x = f2pack(v[e], v[e + 1]), q = fmul2(x, i2);
+        unpack2(ffma2(ffma2(q, l2, ffma2(q, h2, x)), i2, q), v[e], v[e + 1]);
       }
     } else {
 #pragma unroll
@@ -122,7 +130,7 @@ __global__ void __launch_bounds__(1024) rms_norm_q_vec(const RnqArgs a) {
   if (MODE == kShared)
     for (int g = tid; g < a.groups; g += nt) gmax[g] = 0u;
   float h[KV][8];
-  float ss = 0.0f;
+  uint64_t ss2 = 0; // sums of the even and of the odd columns
 #pragma unroll
   for (int k = 0; k < KV; ++k) {
     const int v = tid + k * nt;
@@ -133,18 +141,25 @@ __global__ void __launch_bounds__(1024) rms_norm_q_vec(const RnqArgs a) {
         if (!kAhead) rr[k].load(static_cast<const T *>(a.res) + base + 8 * v);
         rr[k].get(r);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[k][e] += r[e];
+        for (int e = 0; e < 8; e += 2)
+          unpack2(fadd2(f2pack(h[k][e], h[k][e + 1]), f2pack(r[e], r[e + 1])), h[k][e], h[k][e + 1]);
       }
       if (a.sum) Raw8<T>::store(static_cast<T *>(a.sum) + base + 8 * v, h[k]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(h[k][e], h[k][e], ss);
+      for (int e = 0; e < 8; e += 2) {
+        const uint64_t x = f2pack(h[k][e], h[k][e + 1]);
+        ss2 = ffma2(x, x, ss2);
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[k][e] = 0.0f;
     }
   }
-  ss = block_sum(ss, red_f);
+  float ss, odd;
+  unpack2(ss2, ss, odd);
+  ss = block_sum(ss + odd, red_f);
   const Rms r(ss, a.width, a.eps);
+  const uint64_t p2 = f2pack(r.p2, r.p2);
   uint32_t m[KV];
 #pragma unroll
   for (int k = 0; k < KV; ++k) {
@@ -154,10 +169,10 @@ __global__ void __launch_bounds__(1024) rms_norm_q_vec(const RnqArgs a) {
       if (!kAhead) wr[k].load(static_cast<const T *>(a.w) + 8 * (tid + k * nt));
       wr[k].get(w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        h[k][e] = h[k][e] * r.p2 * w[e];
-        m[k] = max(m[k], mag(h[k][e]));
-      }
+      for (int e = 0; e < 8; e += 2)
+        unpack2(fmul2(fmul2(f2pack(h[k][e], h[k][e + 1]), p2), f2pack(w[e], w[e + 1])), h[k][e], h[k][e + 1]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m[k] = max(m[k], mag(h[k][e]));
     }
   }
   // m: the largest magnitude of the group that vector k lies in
