@@ -12,8 +12,8 @@
 // n itself is never formed: 1 / sqrt(...) is split into a power of two, which scales h exactly, and a
 // rest in [1, 2) that only the scale takes, so a code is h w over the largest h w and carries the
 // rounding of h w and of the quotient alone.
-// Measured: 8192 x 4096 BFLOAT16 with residual and FLOAT8 codes 45 us, 5.2 TB/s; one such row 2.4 us
-// in a graph.
+// Measured: 8192 x 4096 BFLOAT16 with residual and FLOAT8 codes 44 us, 5.3 TB/s (in a graph 40, and 32
+// without residual, where the issue slots bind); one such row 2.5 us in a graph.
 #include "attn_math.cuh"
 #include "quant8.cuh"
 
@@ -273,7 +273,8 @@ template <typename T, typename Q> int launch(const RnqArgs &a, int64_t rows, cud
                    (!a.res || aligned(a.res, 16)) && (!a.sum || aligned(a.sum, 16)) &&
                    aligned(a.w, 16) && aligned(a.y, 8);
   if (vec) {
-    // Vectors per thread: 2 up to a width of 16384, then 4.
+    // Vectors per thread: 2 up to a width of 16384, then 4.  One up to a width of 8192 is slower where rows
+    // count (8192 x 4096 in a graph 49 us against 42) and 0.1 us faster for a single row.
     const int nv = a.width / 8, kv = nv <= 32 ? 1 : nv <= 2048 ? 2 : 4;
     const int threads = ((nv + kv - 1) / kv + 31) / 32 * 32;
     if (kv == 1) return launch_vec<T, Q, 1>(a, rows, threads, st);
