@@ -559,7 +559,8 @@ __global__ void __launch_bounds__(CP_THREADS, 1)
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[c * 16 + e] = seen >> e & 1u ? v[c * 16 + e] : -INFINITY;
             poison = poison || (seen != 0u && inv[c] != inv[c]); // it sees values that are not finite
-            if (inv[c] != inv[c]) inv[c] = 0.0f;
+            // its infinite offset must not meet the -inf of the rows that do not see them
+            if (inv[c] != inv[c]) inv[c] = lv[c] = 0.0f;
             vk[c] = 1.0f;
           }
         }

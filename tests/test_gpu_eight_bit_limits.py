@@ -1,0 +1,68 @@
+"""The operators of a decoder step with 8-bit activations and cache at the ends of their ranges:
+scales that are not finite, very large or subnormal, mis-declared buffers, large batches.
+
+Tolerances are those of test_gpu_eight_bit_step, or derived at the test.
+"""
+import math
+
+import pytest
+import torch
+
+from test_gpu_eight_bit_step import (QMAX, TYPES, assert_codes, check_attention,  # noqa: F401
+                                     clean_status, gen, half_step, kind_of, make_cache, reference,
+                                     storage, values)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------
+# Scales that are not finite
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("name", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("rows", [1, 3, 160])
+@pytest.mark.parametrize("head,page", [(128, 16), (64, 64), (40, 10)])
+def test_attention_scales_not_finite_reach_only_what_sees_them(b2, head, page, rows, name, value):
+    """A page whose scale is NaN or infinite (its codes are zeros then, as the append leaves them)
+    makes the queries that see it NaN and no other."""
+    total, window = 400 + rows, 60
+    q = torch.randn(1, 2, rows, head, generator=gen(5), device="cuda").half()
+    attrs = b2.CacheAttributes(left_window_size=window, sink_tokens=3)
+    for block in (300 // page, (total - 1) // page):  # before every window; the last token's
+        cache = make_cache(b2, "fp8", [total], [0], 1, head, page, seed=12)
+        cache.lengths.fill_(400)
+        clean, _ = reference(cache, q, [rows], window=window, sinks=3)
+        at = int(cache.block_table[0, block])
+        getattr(cache, name)[at] = value
+        if math.isinf(value):
+            getattr(cache, name[0])[at] = 0
+        y = b2.QuantizedCacheAttention()(q, cache, attrs)
+        first = rows if block == 300 // page else max(0, block * page - 400)  # that sees the page
+        assert bool(torch.isnan(y[:, :, first:]).all())
+        assert bool(torch.isfinite(y[:, :, :first]).all())
+        if first:
+            err, size = (y.double() - clean)[:, :, :first].norm(), clean[:, :, :first].norm()
+            assert float(err / size) < 2e-3
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("rows", [12, 300])
+def test_prompt_with_a_value_not_finite(b2, rows, value, codes):
+    """One value of a prompt's last page is not finite: earlier queries do not notice."""
+    x = torch.randn(2, 1, 2, rows, 128, generator=gen(rows), device="cuda").half()
+    q = torch.randn(1, 8, rows, 128, generator=gen(1), device="cuda").half()
+    ys = []
+    for bad in (False, True):
+        cache = b2.QuantizedKVCache.allocate(1, 2, rows, 128, page_size=16, dtype=kind_of(b2, codes))
+        v = x[1].clone()
+        if bad:
+            v[0, 1, rows - 1, 7] = value
+        b2.KVCacheAppend()(x[0], v, cache)
+        ys.append(b2.QuantizedCacheAttention()(q, cache))
+    first = (rows - 1) // 16 * 16  # the first query that sees the last page
+    assert torch.equal(ys[0][:, :, :first], ys[1][:, :, :first])
+    assert torch.equal(ys[0][:, :4], ys[1][:, :4])  # the other KV head's
+    assert bool(torch.isnan(ys[1][:, 4:, first:]).all())
