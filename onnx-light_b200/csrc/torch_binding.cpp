@@ -48,6 +48,18 @@ int32_t onnx_type(at::ScalarType t) {
   }
 }
 
+// Bits of an element of an ONNX type as the framework's tensors store it; 0: none of them.
+int bits_of(long dtype) {
+  switch (dtype) {
+  case 21: case 22: case 23: return 4;                            // UINT4, INT4, FLOAT4E2M1
+  case 2: case 3: case 9: case 17: case 18: case 19: case 20: return 8; // UINT8, INT8, BOOL, FLOAT8*
+  case 4: case 5: case 10: case 16: return 16;                    // UINT16, INT16, FLOAT16, BFLOAT16
+  case 1: case 6: case 12: return 32;                             // FLOAT, INT32, UINT32
+  case 7: case 11: case 13: return 64;                            // INT64, DOUBLE, UINT64
+  default: return 0;
+  }
+}
+
 bool fail(PyObject *type, const char *message) {
   PyErr_SetString(type, message);
   return false;
@@ -71,6 +83,23 @@ struct Arg {
     d.shape = t.sizes().data();
     return true;
   }
+  // Whether `dims` elements of the declared type lie in the storage, on the type's boundary: the kernels
+  // read and write what the shape says.
+  bool fits(long dtype, Py_ssize_t n) {
+    const int bits = bits_of(dtype);
+    if (!bits) return fail(PyExc_ValueError, "a QTensor's dtype is not a numeric ONNX type");
+    int64_t count = bits;
+    for (Py_ssize_t i = 0; i < n; ++i)
+      if (dims[i] == 0) return true;
+    for (Py_ssize_t i = 0; i < n; ++i)
+      if (__builtin_mul_overflow(count, dims[i], &count))
+        return fail(PyExc_ValueError, "a QTensor's storage is smaller than its shape");
+    if (t.nbytes() < (size_t)(count / 8 + (count % 8 != 0)))
+      return fail(PyExc_ValueError, "a QTensor's storage is smaller than its shape");
+    if (bits > 8 && reinterpret_cast<uintptr_t>(d.data) % (bits / 8) != 0)
+      return fail(PyExc_ValueError, "a QTensor's storage must start on a boundary of its type");
+    return true;
+  }
   // A torch.Tensor, or a QTensor (data, dtype, shape).  `dtype` replaces the type of 8-bit storage.
   bool parse(PyObject *o, int device, int32_t dtype = 0) {
     if (THPVariable_Check(o)) {
@@ -87,20 +116,18 @@ struct Arg {
     } else if (set(THPVariable_Unpack(data), device)) {
       const Py_ssize_t n = PySequence_Size(shape);
       ok = n <= 8 || fail(PyExc_ValueError, "a QTensor has at most 8 dimensions");
-      int64_t count = 1;
       for (Py_ssize_t i = 0; ok && i < n; ++i) {
         PyObject *v = PySequence_GetItem(shape, i);
         dims[i] = v ? PyLong_AsLongLong(v) : -1;
         Py_XDECREF(v);
         ok = !PyErr_Occurred() && (dims[i] >= 0 || fail(PyExc_ValueError, "a QTensor's shape is not negative"));
-        if (ok) count *= dims[i];
       }
+      const long type = ok ? PyLong_AsLong(code) : 0;
+      ok = ok && !PyErr_Occurred() && fits(type, n);
       if (ok) {
-        d.dtype = (int32_t)PyLong_AsLong(code);
+        d.dtype = (int32_t)type;
         d.ndim = (int32_t)n;
         d.shape = dims;
-        ok = !PyErr_Occurred() &&
-             (t.nbytes() >= (size_t)count || fail(PyExc_ValueError, "a QTensor's storage is smaller than its shape"));
       }
     }
     Py_XDECREF(data);

@@ -66,3 +66,57 @@ def test_prompt_with_a_value_not_finite(b2, rows, value, codes):
     assert torch.equal(ys[0][:, :, :first], ys[1][:, :, :first])
     assert torch.equal(ys[0][:, :4], ys[1][:, :4])  # the other KV head's
     assert bool(torch.isnan(ys[1][:, 4:, first:]).all())
+
+
+# ---------------------------------------------------------------------------
+# Buffers declared larger than they are, or off their type's boundary
+# ---------------------------------------------------------------------------
+
+
+def test_declared_types_must_fit_the_storage(b2):
+    """A QTensor's storage is measured by its declared type, and must start on that type's boundary."""
+    f16, f32 = 10, 1
+    raw = torch.zeros(2 * 64, dtype=torch.uint8, device="cuda")
+    small16, small32 = b2.QTensor(raw, f16, (2, 64)), b2.QTensor(raw, f32, (2, 64))
+    x, w = torch.zeros(2, 64, device="cuda").half(), torch.ones(64, device="cuda").half()
+    norm, mm = b2.RMSNormalizationQuantize(), b2.ScaledMatMul()
+    for args, kw in (((small16, w), {}), ((x, w), {"residual": small16}), ((x, w), {"out_sum": small16}),
+                     ((x, b2.QTensor(raw[:64], f16, (64,))), {}),
+                     ((x, w), {"out_scale": b2.QTensor(raw[:7], f32, (2, 1))})):
+        with pytest.raises(ValueError, match="storage is smaller"):
+            norm(*args, **kw)
+    a = torch.zeros(2, 64, dtype=torch.int8, device="cuda")
+    one = torch.ones(1, device="cuda")
+    with pytest.raises(ValueError, match="storage is smaller"):
+        mm(a, b2.QTensor(raw[:2], f32, (2,)), a, one)
+    with pytest.raises(ValueError, match="storage is smaller"):
+        mm(a, one, a, one, out=b2.QTensor(raw[:4], f16, (2, 2)))
+    cache = b2.QuantizedKVCache.allocate(1, 1, 32, 64, page_size=16)
+    kv = torch.zeros(1, 1, 2, 64, device="cuda").half()
+    small = b2.QTensor(raw, f16, (1, 1, 2, 64))
+    for k, v in ((small, kv), (kv, small), (b2.QTensor(raw, f32, (1, 1, 2, 64)), kv)):
+        with pytest.raises(ValueError, match="storage is smaller"):
+            b2.KVCacheAppend()(k, v, cache)
+    with pytest.raises(ValueError, match="storage is smaller"):
+        b2.KVCacheAppend()(kv, kv, cache, new_lengths=b2.QTensor(raw[:1], 6, (1,)))
+    with pytest.raises(ValueError, match="storage is smaller"):
+        b2.QuantizedCacheAttention()(small, cache)
+    with pytest.raises(ValueError, match="storage is smaller"):
+        b2.QuantizedCacheAttention()(kv, cache, out=small)
+    with pytest.raises(ValueError, match="storage is smaller"):
+        norm(small32, torch.ones(64, device="cuda"))
+    # a shape whose count passes 64 bits
+    with pytest.raises(ValueError, match="storage is smaller"):
+        norm(b2.QTensor(raw, f16, (1 << 32, 1 << 32)), w)
+    # off the boundary of its type
+    odd = torch.zeros(4 * 64 + 1, dtype=torch.uint8, device="cuda")[1:]
+    with pytest.raises(ValueError, match="boundary"):
+        norm(b2.QTensor(odd, f16, (2, 64)), w)
+    with pytest.raises(ValueError, match="boundary"):
+        b2.KVCacheAppend()(b2.QTensor(odd, f16, (1, 1, 2, 64)), kv, cache)
+    # a type that has no size
+    with pytest.raises(ValueError, match="dtype"):
+        norm(b2.QTensor(raw, 8, (2, 64)), w)
+    # what fits and lies right runs
+    y = mm(a, b2.QTensor(one.view(torch.uint8), f32, (1,)), b2.QTensor(a.view(torch.uint8), b2.INT8, (2, 64)), one)
+    assert y.shape == (2, 2)
