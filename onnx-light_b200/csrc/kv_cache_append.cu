@@ -136,8 +136,8 @@ __global__ void __launch_bounds__(KA_THREADS) kv_cache_append_kernel(const KaArg
   }
   // ---- the new codes ----
   dst += (int64_t)older * a.D;
+  const Divisor<Q> by(s);
   if constexpr (VEC) {
-    const Divisor by(s);
     auto put = [&](int v, const Raw8<T> &x) {
       float f[8];
       x.get(f);
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(KA_THREADS) kv_cache_append_kernel(const KaArg
     }
   } else {
     for (int v = threadIdx.x; v < nv; v += KA_THREADS)
-      dst[v] = (uint8_t)Code<Q>::enc(__fdiv_rn(ld1<T>(src, at(v)), s));
+      dst[v] = (uint8_t)Code<Q>::enc(by.one(ld1<T>(src, at(v))));
   }
 }
 

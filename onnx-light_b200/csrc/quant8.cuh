@@ -1,8 +1,8 @@
 // 8-bit codes with a scale: INT8 (|code| <= 127) and FLOAT8E4M3FN (|code| <= 448).
 // A code stands for code * scale.  The scale of a group of values is their largest magnitude
 // divided by 127 or 448, the code the value divided by that scale, rounded to nearest even.  A
-// scale of 0 (all values 0), an infinite one and a NaN (a value is not a number) give the code 0
-// wherever the quotient is not a number, so no NaN code is ever written; the scale carries it.
+// scale of 0 (the values are 0, or so small that it rounds to 0), an infinite one and a NaN (a value is
+// not a number) give zero codes, so no NaN code is ever written; the scale carries it.
 #pragma once
 #include <cuda_fp8.h>
 
@@ -20,7 +20,7 @@ template <typename Q> struct Code;
 template <> struct Code<Int8> {
   static constexpr float kMax = 127.0f;
   static __device__ __forceinline__ uint32_t enc(float v) { // NaN -> 0
-    return (uint32_t)__float2int_rn(v) & 0xffu;
+    return (uint32_t)max(-127, min(127, __float2int_rn(v))) & 0xffu;
   }
   static __device__ __forceinline__ float dec(uint32_t c) { return (float)(int8_t)c; }
 };
@@ -54,18 +54,29 @@ template <typename Q> __device__ __forceinline__ uint2 enc8(const float (&v)[8])
   return r;
 }
 
+// Division by one scale.  A scale of a few units of 2^-149 is rounded so coarsely that quotients by it
+// pass 127 or 448 by up to a half; they are held to the largest code.
+template <typename Q> __device__ __forceinline__ float quotient_by_rounded(float v, float s) {
+  return fminf(fmaxf(__fdiv_rn(v, s), -Code<Q>::kMax), Code<Q>::kMax);
+}
+
 // Division of many values by one scale, correctly rounded: with inv the correctly rounded 1 / s,
 // q = x inv is within an ulp or two, x - q s is exact in one FMA, and q + (x - q s) inv rounds to the
 // nearest quotient (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
 // processor", 1990, theorem on division by a correctly rounded reciprocal).  That needs s and inv
 // well inside the normal range; other scales take the division itself, and a scale that is 0, infinite
 // or not a number gives zeros, the code of such a group.
-struct Divisor {
+template <typename Q> struct Divisor {
   float s, inv;
   int kind; // 0 zeros, 1 products, 2 divisions
   __device__ __forceinline__ explicit Divisor(float scale) : s(scale) {
     kind = !(scale > 0.0f && scale < INFINITY) ? 0 : scale > 1e-30f && scale < 1e30f ? 1 : 2;
     inv = kind == 1 ? __frcp_rn(scale) : 0.0f;
+  }
+  __device__ __forceinline__ float one(float v) const {
+    if (kind != 1) return kind == 0 ? 0.0f : quotient_by_rounded<Q>(v, s);
+    const float q = v * inv;
+    return fmaf(fmaf(-q, s, v), inv, q);
   }
   __device__ __forceinline__ void divide(float (&v)[8]) const {
     if (kind == 1) {
@@ -76,7 +87,7 @@ struct Divisor {
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = kind == 0 ? 0.0f : __fdiv_rn(v[e], s);
+      for (int e = 0; e < 8; ++e) v[e] = one(v[e]);
     }
   }
 };

@@ -77,10 +77,14 @@ template <typename Q> struct ByTop {
     hi = __fdiv_rn(t, Code<Q>::kMax);
     kind = !(s > 0.0f && s < INFINITY) ? 0 : hi > 1e-25f && hi < 1e30f ? 1 : 2;
     lo = fmaf(-hi, Code<Q>::kMax, t) * (1.0f / Code<Q>::kMax);
+    if (kind == 2) { // a quotient of v lo and hi; top / 127 may be subnormal, then by the stored scale itself
+      lo = hi < 1e-36f ? rest : 1.0f;
+      hi = hi < 1e-36f ? s : hi;
+    }
     inv = kind == 1 ? __frcp_rn(hi) : 0.0f;
   }
   __device__ __forceinline__ float one(float v) const {
-    if (kind != 1) return kind == 0 ? 0.0f : __fdiv_rn(v, hi);
+    if (kind != 1) return kind == 0 ? 0.0f : quotient_by_rounded<Q>(v * lo, hi);
     const float q = v * inv;
     return fmaf(fmaf(-q, lo, fmaf(-q, hi, v)), inv, q);
   }

@@ -120,3 +120,56 @@ def test_declared_types_must_fit_the_storage(b2):
     # what fits and lies right runs
     y = mm(a, b2.QTensor(one.view(torch.uint8), f32, (1,)), b2.QTensor(a.view(torch.uint8), b2.INT8, (2, 64)), one)
     assert y.shape == (2, 2)
+
+
+# ---------------------------------------------------------------------------
+# Subnormal values: the scale is a few units of 2^-149
+# ---------------------------------------------------------------------------
+
+
+def units(g, *shape):
+    """Whole multiples of 2^-149 up to 700 of either sign, as FLOAT."""
+    n = torch.randint(0, 701, shape, generator=g, device="cuda", dtype=torch.int32)
+    sign = torch.randint(0, 2, shape, generator=g, device="cuda", dtype=torch.int32) * -(1 << 31)
+    return (n | sign).view(torch.float32)
+
+
+UNIT_F32 = 2.0 ** -149
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("head", [64, 33])
+def test_append_subnormal_values(b2, head, codes):
+    """The stored scale is a / 127 or 448 rounded to whole units of 2^-149, so quotients pass 127 by
+    up to a half: codes stay at the largest one and keep their sign."""
+    cache = b2.QuantizedKVCache.allocate(40, 1, 8, head, page_size=8, dtype=kind_of(b2, codes))
+    top = torch.randint(20, 701, (40, 1, 1, 1), generator=gen(head), device="cuda", dtype=torch.int32)
+    bits = units(gen(head + 1), 40, 1, 8, head).view(torch.int32)
+    x = ((bits & 0x7fffffff) % top + 1 | bits & -(1 << 31)).view(torch.float32)
+    b2.KVCacheAppend()(x, x, cache)
+    for pool, sc in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        s = sc[:, 0].double()
+        assert bool(((s - x.double().abs().amax((1, 2, 3)) / QMAX[codes]).abs() <= 0.5 * UNIT_F32).all())
+        want = torch.nan_to_num(x.double() / s[:, None, None, None], nan=0.0, posinf=0.0, neginf=0.0)
+        assert_codes(pool, want, codes, slack=1e-6)
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("width,group", [(256, 0), (256, 64), (240, 24), (99, 0), (99, 9)])
+def test_norm_subnormal_weights(b2, width, group, codes):
+    """n = h / rms * w with w of a few hundred units u = 2^-149.  The kernel rounds n to units twice
+    (the second after a factor below 2): within 1.5 u and 2^-20 of it; the scale once more, within
+    0.6 u; a code is off by half a step and what 1.5 u make in units of the stored scale."""
+    x = torch.randn(64, width, generator=gen(width), device="cuda")
+    w = units(gen(width + 1), width)
+    r = b2.RMSNormalizationQuantize()(x, w, dtype=kind_of(b2, codes), group_size=group)
+    h = x.double()
+    n = (h / torch.sqrt((h * h).mean(-1, keepdim=True) + 1e-5) * w.double()).view(64, -1, group or width)
+    s = r.Y_scale.double().view(64, -1)
+    assert bool(((s - n.abs().amax(-1) / QMAX[codes]).abs() <= 0.6 * UNIT_F32 + 2e-6 * s).all())
+    live = s > 0
+    want = (n / s[..., None].clamp(min=UNIT_F32)).clamp(-QMAX[codes], QMAX[codes])
+    c = values(storage(r.Y)).view(n.shape)
+    bound = half_step(want.abs() + 2, codes) * 1.001 + 1.5 * UNIT_F32 / s[..., None].clamp(min=UNIT_F32) + 1e-3
+    assert bool(((c - want).abs() <= bound)[live].all())
+    assert float(c[~live].abs().sum()) == 0 and bool(live.any())
