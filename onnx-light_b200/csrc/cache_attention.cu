@@ -25,6 +25,7 @@ using namespace q8;
 
 constexpr int CAA_WARPS = 4;
 constexpr int CAA_DMAX = 512;
+constexpr float CAA_DOWN = 0x1p-24f; // of what is summed: the sum of large values passes FLOAT's range before their mean
 
 template <typename T, typename Q>
 __global__ void __launch_bounds__(CAA_WARPS * 32) cache_attn_any(const CaArgs a) {
@@ -86,7 +87,7 @@ __global__ void __launch_bounds__(CAA_WARPS * 32) cache_attn_any(const CaArgs a)
     l = l * corr + ls;
 #pragma unroll
     for (int c = 0; c < CAA_DMAX / 32; ++c) o[c] *= corr;
-    const float pv = seen ? pj * vs : 0.0f;
+    const float pv = seen ? pj * (vs * CAA_DOWN) : 0.0f;
     const unsigned any = __ballot_sync(0xffffffffu, seen);
     for (unsigned rest = any; rest; rest &= rest - 1) {
       const int src = __ffs(rest) - 1;
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(CAA_WARPS * 32) cache_attn_any(const CaArgs a)
     }
   }
   if (bad) atomicExch(&g_cache_attention_status, 1);
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l; // a NaN in l stays
+  const float inv = l == 0.0f ? 0.0f : 1.0f / CAA_DOWN / l; // a NaN in l stays
 #pragma unroll
   for (int c = 0; c < CAA_DMAX / 32; ++c)
     if (c * 32 + lane < a.D) st1<T>(yp, c * 32 + lane, o[c] * inv);

@@ -14,11 +14,12 @@
 // lose low bits); and p * v_scale, relative to the largest such product of the row, so 2^-11 of
 // what it contributes.  The denominator sums the unrounded p.
 //
-// The running reference of a row is m ~ max_j (s_j + log2 v_scale_j): with p_j = 2^(s_j - m + 7) in
-// fp32, p_j v_scale_j is at most 2^15 for every token, however far the pages' scales lie apart, and
-// keeps its 11 bits down to 2^-21 of the largest and below (FLOAT16's normal range ends at 2^-14).
-// log2 v_scale is held to [-60, 110] so that p cannot overflow; a scale below only makes its
-// products smaller.
+// The running reference of a row is m ~ max_j (s_j + log2 v_scale_j): with p_j = 2^(s_j - m + 19) in
+// fp32, p_j times 2^-12 v_scale_j is at most 2^15 for every token, however far the pages' scales lie
+// apart, and keeps its 11 bits down to 2^-21 of the largest and below (FLOAT16's normal range ends at
+// 2^-14).  log2 v_scale is held to [-60, 122]: below, p would overflow (a smaller scale only makes its
+// products smaller); no scale of finite values is above 2^128 / 127.  The 2^12 keeps p, which the
+// denominator sums, normal down to 2^-23 of the largest even there.
 //
 // Data path: tiles of 32 tokens (K and V, 128 bytes a token, 128-byte swizzle) through a TMA ring
 // filled by one producer warp.  Page numbers and scales are fetched for the next 8 to 32 tiles at
@@ -51,7 +52,9 @@ namespace {
 using namespace q8;
 
 constexpr int KEYS = 32; // tokens per tile
-constexpr float CS_TOP = 15.0f, CS_BASE = 7.0f; // log2 of the largest p * v_scale, and after a move of m
+constexpr float CS_TOP = 15.0f, CS_BASE = 7.0f; // log2 of the largest product of p, and after a move of m
+constexpr float CS_UP = 12.0f, CS_UP_F = 4096.0f; // power of two that p carries and its product does not
+constexpr float CS_LV_MIN = -60.0f, CS_LV_MAX = 122.0f; // of log2 v_scale
 constexpr size_t CS_SMEM_MAX = 232448;
 constexpr int CS_CTAS = 160; // at most, one per SM
 
@@ -464,9 +467,9 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
           stop = true;
           break;
         }
-        if (act && !values) // key scale in score units; value scale; its logarithm; validity
-          sc[s * CHUNKS + ch] = make_float4(ks * a.scale * kLog2E, vs, fminf(fmaxf(log2f(vs), -60.0f), 110.0f),
-                                       z0 >= 0 ? 1.0f : 0.0f);
+        if (act && !values) // key scale in score units; value scale times 2^-12; its logarithm; validity
+          sc[s * CHUNKS + ch] = make_float4(ks * a.scale * kLog2E, vs * (1.0f / CS_UP_F),
+                                            fminf(fmaxf(log2f(vs), CS_LV_MIN), CS_LV_MAX), z0 >= 0 ? 1.0f : 0.0f);
         __syncwarp();
         if (act && ch == 0)
           tc::mbar_expect_tx(&full[s], (uint32_t)__popc(have >> lane & ((1u << nch) - 1u)) * chunk_bytes);
@@ -733,7 +736,7 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) ref[nt][e] = (m_run[nt][e] == -INFINITY ? 0.0f : m_run[nt][e]) - CS_BASE;
+          for (int e = 0; e < 2; ++e) ref[nt][e] = (m_run[nt][e] == -INFINITY ? 0.0f : m_run[nt][e]) - (CS_BASE + CS_UP);
         // ---- P^T fragments ----
         uint32_t pb[MT][NT][2];
 #pragma unroll
@@ -836,7 +839,7 @@ __global__ void __launch_bounds__(CsLayout<DP, NT>::THREADS, 1)
       const int rr = pack * RP + r;
       T *y = static_cast<T *>(a.y) + (int64_t)walk.b * a.q_b + (int64_t)(kvh * a.group + rr % a.group) * a.q_h +
              (int64_t)(rr / a.group) * a.q_s + d;
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float inv = l == 0.0f ? 0.0f : CS_UP_F / l;
       uint2 w;
       if constexpr (std::is_same<T, __half>::value) {
         w.x = half2_of(v.x * inv, v.y * inv);

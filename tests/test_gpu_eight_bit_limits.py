@@ -173,3 +173,39 @@ def test_norm_subnormal_weights(b2, width, group, codes):
     bound = half_step(want.abs() + 2, codes) * 1.001 + 1.5 * UNIT_F32 / s[..., None].clamp(min=UNIT_F32) + 1e-3
     assert bool(((c - want).abs() <= bound)[live].all())
     assert float(c[~live].abs().sum()) == 0 and bool(live.any())
+
+
+# ---------------------------------------------------------------------------
+# Value scales near the top of the range
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows", [1, 6, 140])
+@pytest.mark.parametrize("head,page", [(128, 16), (64, 32), (256, 16), (40, 10)])
+def test_attention_large_value_scales(b2, head, page, rows):
+    """Values up to 8e37, also beside pages of values 2^90 below: sums of products stay finite."""
+    cache = make_cache(b2, "int8", [500 + rows], [0], 1, head, page, seed=8)
+    cache.lengths.fill_(500)
+    pages = cache.block_table[0].long()
+    pages = pages[pages < cache.v_scale.shape[0]]
+    q = torch.randn(1, 4, rows, head, generator=gen(3), device="cuda").bfloat16()
+    ordinary = cache.v_scale[pages]
+    cache.v_scale[pages] = ordinary * 2.0 ** 124  # 2^117 to 2^119
+    check_attention(b2, cache, q)
+    cache.v_scale[pages[1::3]] = ordinary[1::3] * 2.0 ** 34
+    check_attention(b2, cache, q)
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("rows", [1, 6, 140])
+@pytest.mark.parametrize("head,page", [(128, 16), (64, 32), (256, 16), (40, 10)])
+def test_attention_of_values_near_the_largest(b2, head, page, rows, codes):
+    """Values of 1e38 to 3e38, as the append quantizes them: their mean is as large, their sum is not
+    a FLOAT any more."""
+    total = 300 + rows
+    cache = b2.QuantizedKVCache.allocate(1, 1, total, head, page, kind_of(b2, codes))
+    k = torch.randn(1, 1, total, head, generator=gen(1), device="cuda").bfloat16()
+    v = ((1 + 2 * torch.rand(1, 1, total, head, generator=gen(2), device="cuda")) * 1e38).bfloat16()
+    b2.KVCacheAppend()(k, v, cache)
+    cache.lengths.fill_(300)
+    check_attention(b2, cache, torch.randn(1, 4, rows, head, generator=gen(3), device="cuda").bfloat16())
