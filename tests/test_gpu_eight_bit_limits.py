@@ -209,3 +209,79 @@ def test_attention_of_values_near_the_largest(b2, head, page, rows, codes):
     b2.KVCacheAppend()(k, v, cache)
     cache.lengths.fill_(300)
     check_attention(b2, cache, torch.randn(1, 4, rows, head, generator=gen(3), device="cuda").bfloat16())
+
+
+# ---------------------------------------------------------------------------
+# Large batches: the split kernel's ways to share the keys out
+# ---------------------------------------------------------------------------
+
+
+def many_sequences(b2, batch, Hkv, Hq, rows, head, page, longest, codes, seed):
+    """Short sequences of different lengths, some without new tokens or with nothing before them."""
+    g = gen(seed)
+    past = torch.randint(0, longest + 1, (batch,), generator=g, device="cuda", dtype=torch.int32)
+    past[torch.rand(batch, generator=g, device="cuda") < 0.2] = 0
+    past[batch // 2] = longest
+    new = torch.randint(0, rows + 1, (batch,), generator=g, device="cuda", dtype=torch.int32)
+    new[batch - 1] = rows
+    per = -(-(longest + rows) // page)
+    pages = batch * per
+    order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32).view(batch, per)
+    cache = b2.QuantizedKVCache.allocate(batch, Hkv, per * page, head, page, kind_of(b2, codes), pages=pages,
+                                         block_table=order)
+    for pool in (cache.k, cache.v):
+        v = torch.randn(pool.shape, generator=g, device="cuda") * (40.0 if codes == "int8" else 120.0)
+        pool.copy_(v.round().clamp(-127, 127) if codes == "int8" else
+                   v.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8))
+    for sc in (cache.k_scale, cache.v_scale):
+        sc.copy_(torch.rand(sc.shape, generator=g, device="cuda") * 0.02 + 0.01)
+    cache.lengths.copy_(past)
+    q = torch.randn(batch, Hq, rows, head, generator=g, device="cuda").half()
+    return cache, q, new
+
+
+def check_many(b2, cache, q, new, window=-1, sinks=0):
+    batch, Hq, rows, head = q.shape
+    Hkv, page = cache.k.shape[1:3]
+    sides = []
+    for pool, sc in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        ids = cache.block_table.long()
+        v = values(pool[ids]) * sc[ids].double()[..., None, None]
+        sides.append(v.transpose(1, 2).reshape(batch, Hkv, -1, head))
+    k, v = sides
+    at = torch.arange(rows, device="cuda")
+    j = torch.arange(k.shape[2], device="cuda")
+    p = (cache.lengths[:, None] + at)[:, None, :, None]
+    seen = (j <= p) & (at < new[:, None])[:, None, :, None]
+    if window >= 0:
+        seen = seen & ((p - j <= window) | (j < sinks))
+    z = (q.double().view(batch, Hkv, -1, head) @ k.transpose(-1, -2)).view(batch, Hq, rows, -1) / math.sqrt(head)
+    prob = torch.nan_to_num(torch.softmax(z.masked_fill(~seen, -math.inf), -1), nan=0.0).view(batch, Hkv, -1, len(j))
+    want, size = (prob @ x for x in (v, v.abs()))
+    y = b2.QuantizedCacheAttention()(q, cache, b2.CacheAttributes(left_window_size=window, sink_tokens=sinks),
+                                     new_lengths=new)
+    err = (y.double().view_as(want) - want).abs()
+    limit = 2.0 ** -11 * want.abs() * 1.001 + (2.0 ** -11 + 3e-4) * size + 2.0 ** -25
+    assert bool((err <= limit).all()), float((err / limit).max())
+    assert torch.equal(y, b2.QuantizedCacheAttention()(
+        q, cache, b2.CacheAttributes(left_window_size=window, sink_tokens=sinks), new_lengths=new))
+
+
+MANY = [  # batch, KV heads, query heads, rows, head, page, longest
+    (33, 1, 1, 1, 128, 16, 900), (33, 8, 8, 1, 64, 16, 300), (100, 1, 4, 1, 128, 64, 700), (147, 1, 1, 2, 64, 8, 130),
+    (192, 8, 8, 1, 128, 16, 90), (192, 1, 1, 12, 128, 16, 200), (256, 1, 1, 12, 64, 16, 100),
+    (256, 8, 16, 1, 64, 32, 100), (257, 1, 12, 1, 128, 16, 100), (384, 1, 1, 1, 128, 16, 200),
+    (385, 1, 1, 1, 64, 16, 300), (385, 8, 8, 1, 64, 16, 40), (500, 1, 1, 9, 256, 16, 60), (500, 8, 32, 1, 128, 16, 60),
+    (2100, 8, 8, 1, 64, 16, 40), (2100, 8, 16, 2, 64, 8, 70), (32, 16, 16, 530, 144, 16, 60)]
+
+
+@pytest.mark.parametrize("batch,Hkv,Hq,rows,head,page,longest", MANY)
+def test_attention_many_sequences(b2, batch, Hkv, Hq, rows, head, page, longest):
+    """Ranges worked out per warp (up to 32 sequences), per block, and in runs past a block's
+    threads; CTAs of one pair each, ranges that cut pairs, and, with more pairs than counters (about
+    16380), ranges of whole pairs."""
+    codes = "int8" if batch % 2 else "fp8"
+    cache, q, new = many_sequences(b2, batch, Hkv, Hq, rows, head, page, longest, codes, batch + Hkv)
+    check_many(b2, cache, q, new)
+    check_many(b2, cache, q, new, window=longest // 4, sinks=2)
+    check_many(b2, cache, q, torch.zeros_like(new))
