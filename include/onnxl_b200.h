@@ -314,9 +314,10 @@ B2_API int b2_swiglu(const b2_tensor *a, const b2_tensor *b, float alpha, b2_ten
  * A decoder step with 8-bit activations and an 8-bit KV cache.  Codes are INT8
  * (|code| <= 127) or FLOAT8E4M3FN (|code| <= 448) and stand for code * scale;
  * the scale of a group of values is its largest magnitude / 127 or / 448, the
- * code round(value / scale), nearest even.  A group of zeros has scale 0; a
- * NaN or an infinity in a group makes its scale NaN or infinite and leaves no
- * NaN code.  No counterpart in onnx-light.
+ * code round(value / scale), nearest even, at most 127 or 448.  A group of
+ * zeros, or of values so small that their scale rounds to 0, has scale 0 and
+ * zero codes; a NaN or an infinity in a group makes its scale NaN or infinite
+ * and the codes written zeros.  No counterpart in onnx-light.
  */
 
 /*
@@ -396,10 +397,21 @@ typedef struct b2_cache_attention_attrs {
  *    heads * head_size], heads a multiple of the cache's kv_heads;
  *  new_lengths: as in b2_kv_cache_append; y: q's dtype and shape.
  * A query that sees no key, and every row past new_lengths[b], gives 0.
- * Scores, softmax and sums are fp32.  Codes in rows that hold no token of the
+ * Scores, the softmax's maximum and sums and the sums of values are fp32.  Two
+ * things are held in FLOAT16 where the tensor cores take the call (head sizes
+ * that are multiples of 16 up to 256, pages of whole 8s, aligned buffers; other
+ * calls stay in fp32 throughout).  The product of a probability and its page's
+ * value scale is rounded to it: 2^-11 relative, and 2^-32 of the row's largest
+ * where it is smaller than that.  BFLOAT16 queries become FLOAT16 after a power
+ * of two per row, and columns 2^-14 below the row's largest lose low bits.
+ * Exponentials are then the hardware's (2^-22 relative), and value scales below
+ * 2^-60 lose bits gradually.
+ *
+ * Codes in rows that hold no token of the
  * sequence are never used, whatever they are; within its tokens a
  * FLOAT8E4M3FN code must be a number (b2_kv_cache_append writes no other; a
- * NaN among the values is carried by the page's scale).  Lengths past the table
+ * NaN among the values is carried by the page's scale, which reaches the
+ * queries that see a token of the page and no other).  Lengths past the table
  * are cut to it and pages numbered outside the pool are skipped;
  * b2_kernel_status reports either.
  */

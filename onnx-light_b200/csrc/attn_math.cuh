@@ -5,8 +5,8 @@
 
 namespace b2 {
 
-// 2^x with the hardware approximation (relative error about 2^-22; inputs are
-// <= 8 here, and -inf gives 0).
+// 2^x with the hardware approximation (relative error about 2^-22; inputs stay
+// below 128, results below 2^-126 and that of -inf are 0).
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

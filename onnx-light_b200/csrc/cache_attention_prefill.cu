@@ -17,8 +17,11 @@
 // factor and log2 of the value scale part of its offset, p' = 2^(s k_scale + log2 v_scale - m), so O
 // sums p' code and the denominator sums p' / v_scale, one multiplication per 16 keys.  m follows
 // the row's largest exponent lazily: it is moved only when p' would pass 2^15, then to 2^7, and O
-// and l are rescaled; p' in FLOAT16 keeps 11 bits down to 2^-21 of the row's largest and more.
-// BFLOAT16 queries become FLOAT16 after a power of two per row (8 significant bits fit in 11).
+// and l are rescaled; p' in FLOAT16 keeps 11 bits down to 2^-21 of the row's largest and more.  In fp32
+// p' ends at 2^-126, so a page whose value scale is 2^-110 of another's leaves keys of less than about
+// 2^-23 of the row's largest weight out of the denominator.
+// BFLOAT16 queries become FLOAT16 after a power of two per row (8 significant bits fit in 11; columns
+// 2^-14 below the row's largest lose low bits).
 //
 // Every mbarrier is waited phase by phase by the threads that depend on it, and no barrier can run
 // two phases ahead of a waiter.  All waits are bounded; after a time-out the CTA records a code,

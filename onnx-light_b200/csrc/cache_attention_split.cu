@@ -5,7 +5,8 @@
 //
 // A KV head's queries -- the heads of its group times the new positions, a pack of 8 NT rows -- are
 // the 8-wide N side of mma.sync m16n8k16 and the tokens (Q.K) or head columns (P.V) its 16-row M side,
-// so a code read from HBM serves all of them and no MMA row is padding:
+// so a code read from HBM serves all of them and the padding is at most 7 columns of N (half of them for
+// one position of a group of 4 heads):
 //   S^T[16 tokens x 8 rows] += K[16 x 16 columns] Q^T     O^T[16 columns x 8 rows] += V^T[16 x 16 tokens] P^T
 // Codes become FLOAT16 in registers, exactly (INT8 and FLOAT8E4M3FN values both fit), and the page
 // scales multiply in fp32: the key scale the score, the value scale the probability.  Sums and the
@@ -22,8 +23,8 @@
 // denominator sums, normal down to 2^-23 of the largest even there.
 //
 // Data path: tiles of 32 tokens (K and V, 128 bytes a token, 128-byte swizzle) through a TMA ring
-// filled by one producer warp.  Page numbers and scales are fetched for the next 8 to 32 tiles at
-// once, one page chunk a lane; the first tiles' copies start before their scales arrive.  Each
+// filled by two producer warps, one for the keys and scales and one for the values.  Page numbers and
+// scales are fetched for the next 8 to 32 tiles at once, one page chunk a lane; the first tiles' copies start before their scales arrive.  Each
 // tile is one consumer warp's: the swizzle makes the fragment reads (16 bytes a lane) free of
 // bank conflicts, for K along a token's columns and for V across four tokens.
 //
@@ -33,9 +34,9 @@
 // by its last arriver in CTA order, so results do not depend on timing.
 //
 // Measured (32 / 8 heads of 128): 32 sequences of up to 8192 tokens (344 MB of codes)
-// 75.7 us, 4.5 TB/s; 8 sequences with a
-// window of 4096 28.7 us, 2.3 TB/s; one sequence of 4097 tokens 13.3 us.  The consumer warps' dependent
-// chain per tile (widen, MMA, exponentials) bounds the first two, the walk's fixed start and merge the last.
+// 75.7 us, 4.5 TB/s; 8 sequences with a window of 4096 28.7 us, 2.3 TB/s; one sequence of 4097 tokens
+// 13.3 us.  The consumer warps' dependent chain per tile (widen, MMA, exponentials) bounds the first two,
+// the walk's fixed start and merge the last.
 #include <algorithm>
 
 #include "attn_math.cuh"

@@ -67,8 +67,9 @@ template <typename Q> __device__ __forceinline__ float scale_of(uint32_t top, fl
 
 // Quotients by top / 127 or 448, kept as the sum of two floats: q = v inv is within some ulps,
 // v - q (hi + lo) comes from two FMAs, and q + that * inv is the quotient rounded once, but for a
-// second-order term.  A ratio next to a tie between two codes so falls on the side where the inputs
-// put it.  Zeros where the group's scale is 0, infinite or not a number.
+// second-order term.  A ratio next to a tie between two codes so mostly falls on the side where the
+// inputs put it: of 10^8 FLOAT8 codes 204 are a neighbour of the exact one (311 by the rounded scale's
+// chain), of INT8 codes 33 (40).  Zeros where the group's scale is 0, infinite or not a number.
 template <typename Q> struct ByTop {
   float hi, lo, inv;
   int kind; // 0 zeros, 1 products, 2 divisions

@@ -129,9 +129,12 @@ template <typename T, typename Q> int pick(const SmArgs &g, cudaStream_t st) {
 
 } // namespace
 
-// Against the tcgen05 kernel (us, K x N, here / there): INT8 16 rows 4096 x 11008 14.8 / 17.6, 32 rows
-// 19.7 / 12.3; FLOAT8, whose mma.sync is slower, 8 rows 14.1 / 17.7, 16 rows 18.9 / 17.8; with a
-// weight of a million codes, where a launch counts, 32 rows 2.8 / 4.2, 64 rows 5.0 / 4.5.
+// Against the tcgen05 kernel (us in a graph with weights from HBM, K x N, here / there).  Up to two
+// million codes, where a launch counts: 32 rows 1024 x 1024 3.1 / 4.1, 4096 x 512 4.9 / 7.2.  4096 x 4096:
+// INT8 1 row 5.4 / 9.4, 16 rows 6.2 / 8.4, 32 rows 8.0 / 8.3; FLOAT8, whose mma.sync is slower, 8 rows
+// 6.1 / 8.8, 16 rows 8.6 / 8.6, 32 rows 11.8 / 8.5.  4096 x 11008: INT8 1 row 11.9 / 12.2, 16 rows
+// 15.0 / 12.1; FLOAT8 1 row 13.0 / 12.4, 8 rows 14.5 / 12.4.  So the limits of 16 and 8 rows hold for
+// weights of some ten million codes and are up to 3 us late for the largest.
 bool scaled_skinny_eligible(const SmArgs &g, bool f8) {
   const int64_t rows = g.N * g.K <= (1 << 21) ? 32 : f8 ? 8 : 16;
   return g.M <= rows && g.K > 0 && g.K % 16 == 0 && aligned(g.a, 16) && aligned(g.w, 16) &&

@@ -163,7 +163,8 @@ at::Tensor empty_like_shape(at::IntArrayRef shape, at::ScalarType type, int devi
 
 // One zeroed buffer per (device, stream), grown on demand: calls on one stream are ordered, and
 // every call leaves its counters at zero.  A call that is being captured into a graph gets its own
-// buffer, whose counters the graph clears, since a replay may run beside calls on any stream.
+// buffer, which the graph clears (the whole of it, counters and partial results), since a replay may run
+// beside calls on any stream.
 std::map<std::pair<int, cudaStream_t>, at::Tensor> g_workspaces;
 
 void *workspace(int device, cudaStream_t st, size_t need, at::Tensor *keep) {

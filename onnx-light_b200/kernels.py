@@ -522,7 +522,9 @@ class QuantizedCacheAttention:
 
     ``Q``: FLOAT16 / BFLOAT16 [batch, heads, new, head_size] or [batch, new, heads * head_size];
     query i of sequence b stands at position lengths[b] + i.  Call after KVCacheAppend of the same
-    tokens and before ``cache.advance``.  Rows past ``new_lengths`` give 0.
+    tokens and before ``cache.advance``.  Rows past ``new_lengths`` give 0.  Scores, softmax statistics
+    and sums are fp32; probabilities (and BFLOAT16 queries, scaled by row) are FLOAT16 on the tensor
+    cores, as the C header states.
     """
 
     name = "onnx_kernels:GPU:b200:QuantizedCacheAttention"
