@@ -150,13 +150,6 @@ bool checked(int rc) {
   return false;
 }
 
-bool device_of(PyObject *o, int *device) {
-  Arg a;
-  if (!a.parse(o, -1)) return false;
-  *device = a.t.get_device();
-  return true;
-}
-
 at::Tensor empty_like_shape(at::IntArrayRef shape, at::ScalarType type, int device) {
   return at::detail::empty_cuda(shape, type, at::Device(at::kCUDA, (c10::DeviceIndex)device), std::nullopt);
 }
